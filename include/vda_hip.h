@@ -355,6 +355,93 @@ int vda_colormap_bytes_u8(const uint8_t* g, const uint8_t* remap, const uint8_t*
 int vda_warp_blend_f32(const float* prev, const float* cur, const float* flow, float* out, int h, int w, float w_cur, float w_prev,
                        void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Operators of a video transformer that works frame by frame: rotary positions, a token cache in 8 bits, attention of new
+ * tokens over it, and the step between two blocks.  No counterpart in the reference.
+ *
+ * vda_rotary_axes: rotary positions with up to three axes (time, height, width).  Row r is a token at pos[r][0..2]; in each of
+ *   its `heads` heads of hd channels the pairs of channels 0 .. n_t-1 turn with the time axis, the next n_h with height, the next
+ *   n_w with width: pair j by pos[axis(j)] * freq[j] radians, (a, b) -> (a cos - b sin, b cos + a sin).  With n = n_t + n_h + n_w
+ *   pair j is channels (j, j + n) for VDA_PAIR_HALVES and (2j, 2j + 1) for VDA_PAIR_ADJACENT; channels 2n .. hd-1 stay.  A
+ *   token at (0, 0, 0) is unchanged (class tokens); negated frequencies undo a rotation.  q and k that lie side by side in a
+ *   row are turned by one call (heads = both together).
+ *   x, out: dtype BF16, F16 or F32, [rows][ldx] and [rows][ldo] (elements); out may be x itself (with ldo == ldx) and must not
+ *   overlap it otherwise.  pos: int32 [rows][3], or fp32 where pos_float is set; freq: float64 [n].  Angles are formed in
+ *   double, the rotation in fp32.  n % 4 == 0, hd % 8 == 0, hd <= 256; rows 16-byte aligned (in place and 16-bit
+ *   VDA_PAIR_HALVES: 8-byte), else VDA_ESHAPE.
+ * ------------------------------------------------------------------------------------------------------------- */
+enum { VDA_PAIR_HALVES = 0, VDA_PAIR_ADJACENT = 1 };
+int vda_rotary_axes(const void* x, void* out, const void* pos, const double* freq, long rows, int heads, int hd, long ldx, long ldo,
+                    int n_t, int n_h, int n_w, int pairing, int pos_float, int dtype, void* stream);
+
+/* A cache of keys and values in 8 bits, in pages of page_size slots (one page per frame, say).  Planes k and v hold codes,
+ * [pages][kv_heads][page_size][row] with row = hd rounded up to a multiple of 16 bytes (the padding is zero); k_exp and v_exp
+ * [pages][kv_heads][page_size] hold each row's exponent byte e: a stored value is code * 2^(e - 127).  Codes are e4m3 (magnitudes
+ * up to 448) or signed 8-bit integers (-127 .. 127).  A row's e is the smallest (at least 1) that brings its largest magnitude
+ * within the largest code; each code is then the value rounded once, to nearest even.  e = 0 marks an empty slot (clear k_exp and
+ * v_exp before use); e = 255 a row that held an infinity or a NaN, which reads back as NaN.
+ * hd % 8 == 0, hd <= 128, page_size % 16 == 0, planes 16-byte aligned, pages * page_size < 2^31, else VDA_ESHAPE. */
+enum { VDA_CACHE_E4M3 = 0, VDA_CACHE_I8 = 1 };
+typedef struct VdaTokenCache {
+    void *k, *v;
+    uint8_t *k_exp, *v_exp;
+    int pages, page_size, kv_heads, hd, format;
+} VdaTokenCache;
+
+/* vda_cache_write: rows k [rows][ldk] and v [rows][ldv] (dtype BF16, F16 or F32, kv_heads * hd values each) go to the slots
+ *   slots[r] = page * page_size + place (int64; a row whose slot is negative or beyond the cache is skipped; the others are
+ *   distinct).  pos != NULL: the keys are turned first, as by vda_rotary_axes with heads of hd channels, in fp32 without a
+ *   rounding in between.  16-byte aligned rows.
+ * vda_cache_read: the values of the slots, rounded to dtype, into rows k and v; rows without a slot stay as they were, empty
+ *   slots read as 0. */
+int vda_cache_write(const VdaTokenCache* cache, const void* k, const void* v, const int64_t* slots, long rows, long ldk, long ldv, int dtype,
+                    const void* pos, const double* freq, int n_t, int n_h, int n_w, int pairing, int pos_float, void* stream);
+int vda_cache_read(const VdaTokenCache* cache, const int64_t* slots, void* k, void* v, long rows, long ldk, long ldv, int dtype, void* stream);
+
+/* vda_cached_attention: softmax(scale * q K^T) V over the cache, for `seqs` sequences at once.  Sequence s has the query rows
+ *   q_start[s] .. q_start[s+1]-1 of q (int32 [seqs + 1], cut to 0 .. rows; at most max_q of them are computed) and the keys
+ *   0 .. kv_len[s]-1, key i in page page_table[s][i / page_size] (int32 [seqs][max_pages]) at place i % page_size.  Row r sees
+ *   the first visible[r] of its sequence's keys (int32 [rows]; NULL: all): a causal mask, by token or by frame.  Keys
+ *   in empty slots and in pages outside 0 .. pages-1 (evicted ones: -1) are not seen by any row.  A row that sees no key is 0.  What
+ *   is not seen has no effect, NaN included.  Query heads h * G .. h * G + G-1 use key head h, G = heads / kv_heads.
+ *   q, out: dtype BF16, F16 or F32, rows of ldq and ldo elements, 16-byte aligned; rows of no sequence are left as they were.
+ *   Scores, softmax and sums are fp32.  16-bit types: products of IEEE halves, the cached values exactly and the probabilities
+ *   rounded to 11 bits; F32: q and the probabilities in two pieces (22 bits).
+ *   work: vda_cached_attention_work bytes of scratch, 16-byte aligned, of no meaning between calls; calls that may run at the
+ *   same time need one each.  Results are the same bits from run to run. */
+typedef struct VdaCachedAttentionArgs {
+    const void* q;
+    void* out;
+    const int32_t *page_table, *kv_len, *q_start, *visible;
+    void* work;
+    long work_bytes, rows, ldq, ldo;
+    int seqs, max_pages, max_q, heads, dtype;
+    float scale;
+} VdaCachedAttentionArgs;
+long vda_cached_attention_work(const VdaTokenCache* cache, int seqs, int max_pages, int max_q, int heads);    /* negative: a VDA_E* code */
+int vda_cached_attention(const VdaTokenCache* cache, const VdaCachedAttentionArgs* args, void* stream);
+
+/* vda_gated_norm: the step between two blocks, x the fp32 residual stream and b a block's output:
+ *     n = post(b) * post_w + post_b;   x_out = resid_scale * x + gate[g] * n;
+ *     y = (pre(x_out) * pre_w + pre_b) * (1 + mod_scale[g]) + mod_shift[g]
+ *   post, pre: VDA_NORM_NONE (the value itself), VDA_NORM_LAYER (biased variance) or VDA_NORM_RMS, eps inside the root.  g = row /
+ *   rows_per_group: gate, mod_scale and mod_shift are [groups][C] (one group: LayerScale; a group per frame: modulation).  Any of the
+ *   fp32 vectors may be NULL (factor 1, summand 0).  b NULL: no update, x_out must be NULL too and y is taken of x.  y NULL: only the
+ *   update.  x_out may be x.  b_type, y_type: BF16, F16 or F32.  C % 4 == 0, C <= 8192, rows aligned to 4 elements, vectors to
+ *   16 bytes, else VDA_ESHAPE. */
+enum { VDA_NORM_NONE = 0, VDA_NORM_LAYER = 1, VDA_NORM_RMS = 2 };
+typedef struct VdaGatedNormArgs {
+    const float* x;
+    const void* b;
+    float* x_out;
+    void* y;
+    const float *post_w, *post_b, *gate, *pre_w, *pre_b, *mod_scale, *mod_shift;
+    long rows, ldx, ldb, ldxo, ldy;
+    int C, rows_per_group, post, pre, b_type, y_type;
+    float resid_scale, eps;
+} VdaGatedNormArgs;
+int vda_gated_norm(const VdaGatedNormArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

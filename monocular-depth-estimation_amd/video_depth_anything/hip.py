@@ -24,7 +24,8 @@ EXPORTS = [
     "vda_im2col_patch14", "vda_assemble_tokens", "vda_temporal_attention", "vda_scale_shift_sums", "vda_solve_scale_shift",
     "vda_affine_blend", "vda_preprocess_u8", "vda_split3", "vda_sample_points", "vda_scale_frames", "vda_minmax_f32", "vda_colorize_u8",
     "vda_colormap_u8", "vda_colorize_zones_u8", "vda_range_focus_f32", "vda_quantize_u8", "vda_histogram_u8", "vda_colormap_bytes_u8",
-    "vda_warp_blend_f32",
+    "vda_warp_blend_f32", "vda_rotary_axes", "vda_cache_write", "vda_cache_read", "vda_cached_attention_work", "vda_cached_attention",
+    "vda_gated_norm",
 ]
 
 
@@ -41,6 +42,31 @@ class GemmArgs(C.Structure):
         ("up_h", C.c_int), ("up_w", C.c_int), ("acc_scale", C.c_float), ("cin_used", C.c_int),
         ("out16", C.c_void_p), ("row_part", C.c_void_p), ("ld16", C.c_int), ("row_stat", C.c_void_p), ("w_colsum", C.c_void_p),
         ("split_out", C.c_int), ("split_scale", C.c_float), ("sat_flag", C.c_void_p), ("ab_pairs", C.c_int),
+    ]
+
+
+class CacheDesc(C.Structure):        # VdaTokenCache
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+        ("pages", C.c_int), ("page_size", C.c_int), ("kv_heads", C.c_int), ("hd", C.c_int), ("format", C.c_int),
+    ]
+
+
+class CachedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("page_table", C.c_void_p), ("kv_len", C.c_void_p), ("q_start", C.c_void_p),
+        ("visible", C.c_void_p), ("work", C.c_void_p), ("work_bytes", C.c_long), ("rows", C.c_long), ("ldq", C.c_long), ("ldo", C.c_long),
+        ("seqs", C.c_int), ("max_pages", C.c_int), ("max_q", C.c_int), ("heads", C.c_int), ("dtype", C.c_int), ("scale", C.c_float),
+    ]
+
+
+class GatedNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("b", C.c_void_p), ("x_out", C.c_void_p), ("y", C.c_void_p), ("post_w", C.c_void_p), ("post_b", C.c_void_p),
+        ("gate", C.c_void_p), ("pre_w", C.c_void_p), ("pre_b", C.c_void_p), ("mod_scale", C.c_void_p), ("mod_shift", C.c_void_p),
+        ("rows", C.c_long), ("ldx", C.c_long), ("ldb", C.c_long), ("ldxo", C.c_long), ("ldy", C.c_long),
+        ("C", C.c_int), ("rows_per_group", C.c_int), ("post", C.c_int), ("pre", C.c_int), ("b_type", C.c_int), ("y_type", C.c_int),
+        ("resid_scale", C.c_float), ("eps", C.c_float),
     ]
 
 
@@ -101,8 +127,16 @@ def lib():
         l.vda_histogram_u8.argtypes = [C.c_void_p, C.c_void_p, C.c_long, C.c_void_p]
         l.vda_colormap_bytes_u8.argtypes = [C.c_void_p] * 4 + [C.c_long, C.c_void_p]
         l.vda_warp_blend_f32.argtypes = [C.c_void_p] * 4 + [C.c_int, C.c_int, C.c_float, C.c_float, C.c_void_p]
+        l.vda_rotary_axes.argtypes = [C.c_void_p] * 4 + [C.c_long, C.c_int, C.c_int, C.c_long, C.c_long] + [C.c_int] * 6 + [C.c_void_p]
+        l.vda_cache_write.argtypes = ([C.POINTER(CacheDesc)] + [C.c_void_p] * 3 + [C.c_long] * 3 + [C.c_int, C.c_void_p, C.c_void_p]
+                                      + [C.c_int] * 5 + [C.c_void_p])
+        l.vda_cache_read.argtypes = [C.POINTER(CacheDesc)] + [C.c_void_p] * 3 + [C.c_long] * 3 + [C.c_int, C.c_void_p]
+        l.vda_cached_attention_work.argtypes = [C.POINTER(CacheDesc)] + [C.c_int] * 4
+        l.vda_cached_attention.argtypes = [C.POINTER(CacheDesc), C.POINTER(CachedAttentionArgs), C.c_void_p]
+        l.vda_gated_norm.argtypes = [C.POINTER(GatedNormArgs), C.c_void_p]
         for name in EXPORTS[1:]:
             getattr(l, name).restype = C.c_int
+        l.vda_cached_attention_work.restype = C.c_long
         _lib = l
     return _lib
 
@@ -545,3 +579,186 @@ def warp_blend_f32(prev, cur, flow, out, h, w, w_cur, w_prev):
     _need("vda_warp_blend_f32", prev=(prev, h * w), cur=(cur, h * w), flow=(flow, 2 * h * w), out=(out, h * w))
     _check(lib().vda_warp_blend_f32(_ptr(prev), _ptr(cur), _ptr(flow), _ptr(out), h, w, float(w_cur), float(w_prev), _stream()),
            "vda_warp_blend_f32")
+
+
+# ---- operators of a video transformer that works frame by frame: rotary positions, token cache, attention over it, norms -----------
+PAIR_HALVES, PAIR_ADJACENT = 0, 1                   # VDA_PAIR_*
+CACHE_E4M3, CACHE_I8 = 0, 1                         # VDA_CACHE_*
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2           # VDA_NORM_*
+
+
+def _here(what, *ts):
+    """These operators launch on the current device's current stream: all tensors have to live there."""
+    _dev(*ts)
+    here = torch.cuda.current_device() if _current_device is None else _current_device()
+    for t in ts:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"{what}: a tensor is on device {t.get_device()}, the current device is {here}")
+
+
+def _row_stride(what, name, t, width, ld):
+    """Elements from one row of ``t`` to the next: ``ld``, or what the tensor's own stride says.  Within a row values are dense."""
+    if t.dim() < 2:
+        return width if ld is None else ld
+    dense = 1
+    for n, s in zip(t.shape[:0:-1], t.stride()[:0:-1]):
+        if n != 1 and s != dense:
+            raise ValueError(f"{what}: the rows of {name} are not dense (strides {tuple(t.stride())})")
+        dense *= n
+    return (max(t.stride(0), width) if t.shape[0] > 1 else width) if ld is None else ld
+
+
+def _axes(what, pos, freq, sections, rows):
+    n_t, n_h, n_w = sections
+    if pos.dtype not in (torch.int32, torch.float32) or freq.dtype != torch.float64:
+        raise TypeError(f"{what}: int32 or fp32 positions, float64 frequencies")
+    if not (pos.is_contiguous() and freq.is_contiguous()):
+        raise ValueError(f"{what}: pos and freq are dense")
+    _need(what, pos=(pos, 3 * rows), freq=(freq, n_t + n_h + n_w))
+    return n_t, n_h, n_w
+
+
+def rotary_axes(x, out, pos, freq, *, rows, heads, hd, sections, pairing=PAIR_HALVES, ldx=None, ldo=None):
+    """Turns the channel pairs of ``heads`` heads of every row of ``x`` by the row's position: ``pos`` int32 or fp32 [rows, 3] =
+    (time, height, width), ``freq`` float64 radians per unit step of each pair, ``sections`` = pairs that follow (time, height,
+    width).  ``out`` may be ``x``.  Row strides are the tensors' own unless given.  A negated ``freq`` undoes the rotation."""
+    what = "vda_rotary_axes"
+    _here(what, x, out, pos, freq)
+    if x.dtype != out.dtype or x.dtype not in _TYPES:
+        raise TypeError(f"{what}: x and out share one type of fp32, bf16, fp16")
+    n_t, n_h, n_w = _axes(what, pos, freq, sections, rows)
+    ldx, ldo = _row_stride(what, "x", x, heads * hd, ldx), _row_stride(what, "out", out, heads * hd, ldo)
+    _need(what, x=(x, (rows - 1) * ldx + heads * hd), out=(out, (rows - 1) * ldo + heads * hd))
+    _check(lib().vda_rotary_axes(_ptr(x), _ptr(out), _ptr(pos), _ptr(freq), rows, heads, hd, ldx, ldo, n_t, n_h, n_w, int(pairing),
+                                 int(pos.dtype == torch.float32), _type(x), _stream()), what)
+
+
+def cache_row_bytes(hd):
+    """Bytes of a row of codes in a cache plane."""
+    return (hd + 15) // 16 * 16
+
+
+def _cache(what, ck, cv, ek, ev, kv_heads, hd, page_size, fmt):
+    shape = (ck.shape[0], kv_heads, page_size, cache_row_bytes(hd))
+    for t, want in ((ck, shape), (cv, shape), (ek, shape[:3]), (ev, shape[:3])):
+        if t.dtype != torch.uint8:
+            raise TypeError(f"{what}: cache planes are uint8")
+        if tuple(t.shape) != want or not t.is_contiguous():
+            raise ValueError(f"{what}: a cache plane of shape {tuple(t.shape)}, wanted dense {want}")
+    return CacheDesc(ck.data_ptr(), cv.data_ptr(), ek.data_ptr(), ev.data_ptr(), shape[0], page_size, kv_heads, hd, int(fmt))
+
+
+def cache_write(k, v, ck, cv, ek, ev, slots, *, rows, kv_heads, hd, page_size, fmt, pos=None, freq=None, sections=None,
+                pairing=PAIR_HALVES, ldk=None, ldv=None):
+    """Quantises rows ``k`` and ``v`` into the cache planes (codes ``ck``, ``cv``, exponents ``ek``, ``ev``) at ``slots`` (int64,
+    page * page_size + place, distinct; negative: the row is skipped).  ``pos``, ``freq``, ``sections``: the keys are turned first, as
+    by ``rotary_axes``."""
+    what = "vda_cache_write"
+    _here(what, k, v, ck, cv, ek, ev, slots, pos, freq)
+    if k.dtype != v.dtype or k.dtype not in _TYPES or slots.dtype != torch.int64:
+        raise TypeError(f"{what}: k and v share one type of fp32, bf16, fp16; slots are int64")
+    if (pos is None) != (freq is None) or (pos is None) != (sections is None):
+        raise ValueError(f"{what}: pos, freq and sections come together")
+    desc = _cache(what, ck, cv, ek, ev, kv_heads, hd, page_size, fmt)
+    n = _axes(what, pos, freq, sections, rows) if pos is not None else (0, 0, 0)
+    width = kv_heads * hd
+    ldk, ldv = _row_stride(what, "k", k, width, ldk), _row_stride(what, "v", v, width, ldv)
+    if not slots.is_contiguous():
+        raise ValueError(f"{what}: slots are dense")
+    _need(what, k=(k, (rows - 1) * ldk + width), v=(v, (rows - 1) * ldv + width), slots=(slots, rows))
+    _check(lib().vda_cache_write(C.byref(desc), _ptr(k), _ptr(v), _ptr(slots), rows, ldk, ldv, _type(k), _ptr(pos), _ptr(freq), *n, int(pairing),
+                                 int(pos is not None and pos.dtype == torch.float32), _stream()), what)
+
+
+def cache_read(ck, cv, ek, ev, slots, k, v, *, rows, kv_heads, hd, page_size, fmt, ldk=None, ldv=None):
+    """The values held at ``slots``, rounded to the type of ``k`` and ``v``; rows with a negative slot stay as they were, empty slots
+    read as 0."""
+    what = "vda_cache_read"
+    _here(what, k, v, ck, cv, ek, ev, slots)
+    if k.dtype != v.dtype or k.dtype not in _TYPES or slots.dtype != torch.int64:
+        raise TypeError(f"{what}: k and v share one type of fp32, bf16, fp16; slots are int64")
+    desc = _cache(what, ck, cv, ek, ev, kv_heads, hd, page_size, fmt)
+    width = kv_heads * hd
+    ldk, ldv = _row_stride(what, "k", k, width, ldk), _row_stride(what, "v", v, width, ldv)
+    if not slots.is_contiguous():
+        raise ValueError(f"{what}: slots are dense")
+    _need(what, k=(k, (rows - 1) * ldk + width), v=(v, (rows - 1) * ldv + width), slots=(slots, rows))
+    _check(lib().vda_cache_read(C.byref(desc), _ptr(slots), _ptr(k), _ptr(v), rows, ldk, ldv, _type(k), _stream()), what)
+
+
+def cached_attention_work(ck, *, seqs, max_pages, max_q, heads, kv_heads, hd, page_size, fmt):
+    """Bytes of scratch that ``cached_attention`` needs for these sizes."""
+    desc = CacheDesc(ck.data_ptr(), ck.data_ptr(), ck.data_ptr(), ck.data_ptr(), ck.shape[0], page_size, kv_heads, hd, int(fmt))
+    n = lib().vda_cached_attention_work(C.byref(desc), seqs, max_pages, max_q, heads)
+    _check(min(n, 0), "vda_cached_attention_work")
+    return n
+
+
+def cached_attention(q, out, ck, cv, ek, ev, page_table, kv_len, q_start, *, heads, kv_heads, hd, page_size, fmt, max_q, scale,
+                     visible=None, work=None, rows=None, ldq=None, ldo=None):
+    """softmax(scale q K^T) V of the query rows of every sequence over its cached keys.  ``page_table`` int32 [seqs, max_pages],
+    ``kv_len`` int32 [seqs], ``q_start`` int32 [seqs + 1] (rows of sequence s: q_start[s] .. q_start[s+1]-1, at most ``max_q``),
+    ``visible`` int32 [rows]: leading keys that a row sees (None: all).  ``work``: uint8 scratch of ``cached_attention_work`` bytes;
+    None takes it from torch's allocator for this call.  Rows of no sequence stay as they were; a row that sees no key is 0."""
+    what = "vda_cached_attention"
+    _here(what, q, out, ck, cv, ek, ev, page_table, kv_len, q_start, visible, work)
+    if q.dtype != out.dtype or q.dtype not in _TYPES:
+        raise TypeError(f"{what}: q and out share one type of fp32, bf16, fp16")
+    for t in (page_table, kv_len, q_start, visible):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise TypeError(f"{what}: page_table, kv_len, q_start and visible are dense int32")
+    if page_table.dim() != 2 or page_table.shape[0] != kv_len.numel() or q_start.numel() != kv_len.numel() + 1:
+        raise ValueError(f"{what}: page_table [seqs, max_pages], kv_len [seqs] and q_start [seqs + 1] belong together")
+    desc = _cache(what, ck, cv, ek, ev, kv_heads, hd, page_size, fmt)
+    seqs, max_pages = page_table.shape
+    width = heads * hd
+    ldq, ldo = _row_stride(what, "q", q, width, ldq), _row_stride(what, "out", out, width, ldo)
+    rows = q.shape[0] if rows is None else rows
+    _need(what, q=(q, (rows - 1) * ldq + width), out=(out, (rows - 1) * ldo + width), visible=(visible, rows))
+    n = lib().vda_cached_attention_work(C.byref(desc), seqs, max_pages, max_q, heads)
+    _check(min(n, 0), what)
+    if work is None:
+        work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    have = 0 if work is None else work.untyped_storage().nbytes() - work.storage_offset() * work.element_size()
+    if have < n:
+        raise ValueError(f"{what}: work holds {have} bytes, the call needs {n}")
+    a = CachedAttentionArgs(q.data_ptr(), out.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(), q_start.data_ptr(),
+                            None if visible is None else visible.data_ptr(), None if work is None else work.data_ptr(), have, rows, ldq, ldo,
+                            seqs, max_pages, max_q, heads, _type(q), float(scale))
+    _check(lib().vda_cached_attention(C.byref(desc), C.byref(a), _stream()), what)
+
+
+def gated_norm(x, b, x_out, y, *, rows, C, post=NORM_NONE, post_w=None, post_b=None, gate=None, resid_scale=1.0, pre=NORM_LAYER, pre_w=None,
+               pre_b=None, mod_scale=None, mod_shift=None, rows_per_group=None, eps=1e-6, ldx=None, ldb=None, ldxo=None, ldy=None):
+    """The step between two blocks: ``x_out = resid_scale * x + gate[g] * (post(b) * post_w + post_b)`` and ``y = (pre(x_out) * pre_w +
+    pre_b) * (1 + mod_scale[g]) + mod_shift[g]``, g = row // rows_per_group (default: one group).  ``x``, ``x_out`` fp32 (may be the
+    same), ``b`` and ``y`` of any storage type; ``b = x_out = None``: y of x alone; ``y = None`` (with pre = NORM_NONE): the update alone."""
+    what = "vda_gated_norm"
+    vectors = dict(post_w=post_w, post_b=post_b, pre_w=pre_w, pre_b=pre_b)
+    grouped = dict(gate=gate, mod_scale=mod_scale, mod_shift=mod_shift)
+    _here(what, x, b, x_out, y, *vectors.values(), *grouped.values())
+    per = rows if rows_per_group is None else rows_per_group
+    if per <= 0:
+        raise ValueError(f"{what}: rows_per_group is positive")
+    groups = -(-rows // per)
+    for name, t in (("x", x), ("x_out", x_out), *vectors.items(), *grouped.items()):
+        if t is not None and t.dtype != torch.float32:
+            raise TypeError(f"{what}: {name} is fp32")
+    for name, t in (*vectors.items(), *grouped.items()):
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{what}: {name} is dense")
+    for t in (b, y):
+        if t is not None and t.dtype not in _TYPES:
+            raise TypeError(f"{what}: b and y are fp32, bf16 or fp16")
+    stride = lambda name, t, ld: C if t is None else _row_stride(what, name, t, C, ld)  # noqa: E731
+    ldx, ldb, ldxo, ldy = stride("x", x, ldx), stride("b", b, ldb), stride("x_out", x_out, ldxo), stride("y", y, ldy)
+    _need(what, x=(x, (rows - 1) * ldx + C), b=(b, (rows - 1) * ldb + C), x_out=(x_out, (rows - 1) * ldxo + C), y=(y, (rows - 1) * ldy + C),
+          **{n: (t, C) for n, t in vectors.items()}, **{n: (t, groups * C) for n, t in grouped.items()})
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    a = GatedNormArgs(p(x), p(b), p(x_out), p(y), p(post_w), p(post_b), p(gate), p(pre_w), p(pre_b), p(mod_scale), p(mod_shift),
+                      rows, ldx, ldb, ldxo, ldy, C, per, int(post), int(pre), T_NONE if b is None else _type(b), T_NONE if y is None else _type(y),
+                      float(resid_scale), float(eps))
+    _check(lib().vda_gated_norm(_byref(a), _stream()), what)
+
+
+_byref = C.byref          # (``C`` is the channel count inside gated_norm)

@@ -1,0 +1,481 @@
+"""Rotary positions, the 8-bit token cache, attention over it and the gated norm, each through the C ABI against its definition in
+64 bits (token_ops_ref.py, which also derives the bounds)."""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import token_ops_ref as R  # noqa: E402
+from video_depth_anything import hip  # noqa: E402
+
+DEV = "cuda"
+HALVES = [torch.bfloat16, torch.float16]
+TYPES = HALVES + [torch.float32]
+PAIR = {"halves": hip.PAIR_HALVES, "adjacent": hip.PAIR_ADJACENT}
+FMT = {"i8": hip.CACHE_I8, "e4m3": hip.CACHE_E4M3}
+NORM = {"none": hip.NORM_NONE, "layer": hip.NORM_LAYER, "rms": hip.NORM_RMS}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def within(got, want, tol, what=""):
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    fine = ~torch.isnan(want)
+    over = ((got - want).abs() - tol)[fine]
+    assert over.numel() == 0 or float(over.max()) <= 0, f"{what}: {float(over.max()):.3e} beyond the bound, of {float(want[fine].abs().max()):.3e}"
+
+
+# ---- rotary positions ------------------------------------------------------------------------------------------------------
+def rotary_inputs(rows, heads, hd, n, dt, seed, far=False, pos_float=False):
+    g = gen(seed)
+    x = torch.randn((rows, heads, hd), generator=g).to(dt).to(DEV)
+    pos = torch.randint(-5_000_000 if far else -40, 5_000_000 if far else 2000, (rows, 3), generator=g)
+    pos = (pos.float() * 0.37 if pos_float else pos.to(torch.int32)).to(DEV)
+    freq = (torch.rand(n, generator=g, dtype=torch.float64) * 2).to(DEV)
+    return x, pos, freq
+
+
+def rotary_check(got, x, pos, freq, sections, pairing):
+    want, size = R.rotate(x, pos, freq, sections, pairing)
+    d = R.ROTATION * size
+    within(got, want, d + (0 if x.dtype == torch.float32 else R.half_step(x.dtype)) * (want.abs() + d) + 2.0 ** -25, pairing)
+
+
+@pytest.mark.parametrize("pairing", ["halves", "adjacent"])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,heads,hd,sections", [(1, 1, 8, (4, 0, 0)), (1, 12, 64, (8, 12, 12)), (37, 6, 64, (0, 8, 8)), (1371, 3, 48, (6, 9, 9)),
+                                                    (2050, 2, 24, (1, 1, 2)), (5, 32, 128, (16, 24, 24)), (66, 5, 96, (4, 20, 16)), (9, 2, 256, (40, 44, 44))])
+def test_rotary_turns_every_pair(rows, heads, hd, sections, dt, pairing):
+    x, pos, freq = rotary_inputs(rows, heads, hd, sum(sections), dt, rows + hd)
+    out = torch.full_like(x, float("nan"))
+    hip.rotary_axes(x, out, pos, freq, rows=rows, heads=heads, hd=hd, sections=sections, pairing=PAIR[pairing])
+    rotary_check(out, x, pos, freq, sections, pairing)
+    y = x.clone()
+    hip.rotary_axes(y, y, pos, freq, rows=rows, heads=heads, hd=hd, sections=sections, pairing=PAIR[pairing])
+    assert torch.equal(y, out)
+
+
+@pytest.mark.parametrize("pos_float", [False, True])
+@pytest.mark.parametrize("dt", TYPES)
+def test_rotary_far_positions(dt, pos_float):
+    """Positions of millions, whose fp32 angles are off by tenths of a radian."""
+    x, pos, freq = rotary_inputs(300, 4, 64, 32, dt, 5, far=True, pos_float=pos_float)
+    out = torch.empty_like(x)
+    hip.rotary_axes(x, out, pos, freq, rows=300, heads=4, hd=64, sections=(10, 11, 11))
+    rotary_check(out, x, pos, freq, (10, 11, 11), "halves")
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_rotary_of_q_and_k_inside_packed_rows(dt):
+    """q and k of a packed [q | k | v] row in one call, in place: v and the rest of the buffer stay bit for bit."""
+    rows, heads, hd = 70, 3, 32
+    buf = torch.randn((rows + 2, 3 * heads * hd + 16), generator=gen(3)).to(dt).to(DEV)
+    was = buf.clone()
+    view = buf[1:rows + 1, :2 * heads * hd]
+    _, pos, freq = rotary_inputs(rows, 1, hd, 16, dt, 4)
+    hip.rotary_axes(view, view, pos, freq, rows=rows, heads=2 * heads, hd=hd, sections=(4, 6, 6))
+    rotary_check(view.reshape(rows, 2 * heads, hd), was[1:rows + 1, :2 * heads * hd].reshape(rows, 2 * heads, hd), pos, freq, (4, 6, 6), "halves")
+    assert torch.equal(buf[:, 2 * heads * hd:], was[:, 2 * heads * hd:]) and torch.equal(buf[0], was[0]) and torch.equal(buf[-1], was[-1])
+
+
+def test_rotary_with_negated_frequencies_is_the_inverse_and_the_gradient():
+    """The rotation is orthogonal: turned back it is the input, and the gradient of <w, rotate(x)> with respect to x is w turned back."""
+    x, pos, freq = rotary_inputs(50, 2, 64, 32, torch.float32, 8)
+    y, z = torch.empty_like(x), torch.empty_like(x)
+    kw = dict(rows=50, heads=2, hd=64, sections=(8, 12, 12))
+    hip.rotary_axes(x, y, pos, freq, **kw)
+    hip.rotary_axes(y, z, pos, -freq, **kw)
+    size = R.rotate(x, pos, freq, (8, 12, 12), "halves")[1]
+    within(z, x.double().cpu(), 4 * R.ROTATION * size)
+    w, gx = torch.randn(x.shape, generator=gen(9)).to(DEV), torch.empty_like(x)
+    hip.rotary_axes(w, gx, pos, -freq, **kw)
+    a = x.double().cpu().requires_grad_(True)
+    (R.rotate(a.detach(), pos, freq, (8, 12, 12), "halves")[0] * 0).sum()
+    step = torch.randn(x.shape, generator=gen(10), dtype=torch.float64)
+    f = lambda v: float((w.double().cpu() * R.rotate(v, pos, freq, (8, 12, 12), "halves")[0]).sum())  # noqa: E731
+    base = x.double().cpu()
+    difference = f(base + step) - f(base)                 # the map is linear: the difference is the derivative
+    assert abs(difference - float((gx.double().cpu() * step).sum())) <= 4 * R.ROTATION * float((w.abs().cpu().double().sum() * step.abs().max()))
+
+
+# ---- the cache ---------------------------------------------------------------------------------------------------------------
+def new_cache(pages, kv_heads, page, hd, fill=0):
+    code = lambda: torch.full((pages, kv_heads, page, hip.cache_row_bytes(hd)), fill, dtype=torch.uint8, device=DEV)  # noqa: E731
+    exps = lambda: torch.zeros((pages, kv_heads, page), dtype=torch.uint8, device=DEV)  # noqa: E731
+    return code(), code(), exps(), exps()
+
+
+def cache_rows(rows, kv_heads, hd, dt, seed):
+    """Rows of very different sizes, some of zeros, of one value, of the type's extremes, with ties between codes."""
+    g = gen(seed)
+    x = torch.randn((rows, kv_heads, hd), generator=g) * torch.exp2(torch.randint(-12, 13, (rows, kv_heads, 1), generator=g).float())
+    x[::7] = torch.round(torch.randn(x[::7].shape, generator=g) * 20) / 2            # halves: ties between neighbouring codes
+    x = x.to(dt)
+    if rows > 3:
+        x[1] = 0
+        x[2, :, 0] = torch.finfo(dt).max
+        x[3] = torch.finfo(dt).tiny
+    return x.to(DEV)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,kv_heads,hd,page", [(1, 1, 8, 16), (1, 6, 64, 1376), (45, 3, 24, 16), (2100, 2, 32, 48), (100, 4, 48, 64), (33, 16, 64, 16),
+                                                   (77, 2, 96, 32), (260, 1, 128, 1376), (50, 5, 16, 16), (20, 3, 40, 32)])
+def test_cache_write_stores_the_rules_codes_and_reads_back(rows, kv_heads, hd, page, dt, fmt):
+    pages = -(-rows // page) + 3
+    slots = torch.randperm(pages * page, generator=gen(rows))[:rows].to(DEV)
+    if rows > 10:
+        slots[4], slots[9] = -1, pages * page + 5                               # rows without a slot
+    k, v = cache_rows(rows, kv_heads, hd, dt, 1), cache_rows(rows, kv_heads, hd, dt, 2)
+    ck, cv, ek, ev = new_cache(pages, kv_heads, page, hd, fill=0xAB)
+    kw = dict(rows=rows, kv_heads=kv_heads, hd=hd, page_size=page, fmt=FMT[fmt])
+    hip.cache_write(k, v, ck, cv, ek, ev, slots, **kw)
+    here = (slots >= 0) & (slots < pages * page)
+    p, o = slots[here] // page, slots[here] % page
+    for x, c, e in ((k, ck, ek), (v, cv, ev)):
+        want_e = R.exponents(x[here].cpu(), fmt)
+        assert torch.equal(e[p, :, o].cpu().long(), want_e)
+        raw = c[p, :, o].cpu()
+        if hd % 16:
+            assert int(raw[..., hd:].max()) == 0                                  # padding
+        got = raw[..., :hd].contiguous().view(torch.int8 if fmt == "i8" else torch.float8_e4m3fn).double()
+        assert torch.equal(got, R.codes(x[here].cpu(), want_e, fmt))
+        untouched = torch.ones(pages, page, dtype=torch.bool)
+        untouched[p.cpu(), o.cpu()] = False
+        assert int((c.cpu().permute(0, 2, 1, 3)[untouched] != 0xAB).sum()) == 0 and int(e.cpu().permute(0, 2, 1)[untouched].sum()) == 0
+    k2, v2 = torch.full_like(k, 7.0), torch.full_like(v, 7.0)
+    hip.cache_read(ck, cv, ek, ev, slots, k2, v2, **kw)
+    for got, c, e in ((k2, ck, ek), (v2, cv, ev)):
+        assert torch.equal(got[here].cpu(), R.decode(c[p, :, o][..., :hd], e[p, :, o], fmt).to(dt))
+        assert bool((got[~here] == 7.0).all())
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("pairing", ["halves", "adjacent"])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,kv_heads,hd,sections", [(1, 2, 64, (8, 12, 12)), (90, 3, 24, (2, 5, 5)), (1100, 2, 128, (16, 24, 24)), (40, 4, 96, (4, 8, 12)),
+                                                       (17, 2, 8, (2, 1, 1))])
+def test_cache_write_turns_the_keys(rows, kv_heads, hd, sections, dt, pairing, fmt):
+    """A stored key is within half a code's step of the turned key; the exponent is the rule's for a row as large as the turned one."""
+    k, pos, freq = rotary_inputs(rows, kv_heads, hd, sum(sections), dt, hd + rows)
+    v = cache_rows(rows, kv_heads, hd, dt, 2)
+    page, pages = 32, -(-rows // 32)
+    ck, cv, ek, ev = new_cache(pages, kv_heads, page, hd)
+    slots = torch.arange(rows, device=DEV)
+    kw = dict(rows=rows, kv_heads=kv_heads, hd=hd, page_size=page, fmt=FMT[fmt])
+    hip.cache_write(k, v, ck, cv, ek, ev, slots, pos=pos, freq=freq, sections=sections, pairing=PAIR[pairing], **kw)
+    want, size = R.rotate(k, pos, freq, sections, pairing)
+    p, o = slots // page, slots % page
+    e = ek[p, :, o].cpu().long()
+    d = R.ROTATION * size
+    low, high = R.exponents(want * (1 - 1e-6), fmt), R.exponents(want * (1 + 1e-6), fmt)
+    assert bool(((e >= low) & (e <= high)).all())
+    scale = torch.exp2(e.double() - 127)[..., None]
+    code = (want / scale).abs()
+    step = torch.ones_like(code) if fmt == "i8" else torch.exp2(torch.floor(torch.log2(code.clamp_min(2.0 ** -6))) - 3)
+    got = R.decode(ck[p, :, o][..., :hd], ek[p, :, o], fmt)
+    within(got, want, step * scale / 2 * (1 + 1e-5) + d)
+    assert torch.equal(ev[p, :, o].cpu().long(), R.exponents(v.cpu(), fmt))
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dt", TYPES)
+def test_cache_rows_with_infinities_and_nans_read_back_as_nan(dt, fmt):
+    k = torch.randn((4, 2, 32), generator=gen(1)).to(dt).to(DEV)
+    v = k.clone()
+    k[0, 0, 5], k[1, 1, 31], v[2, 0, 0], v[3, 1, 7] = math.inf, math.nan, -math.inf, math.nan
+    ck, cv, ek, ev = new_cache(1, 2, 16, 32)
+    slots = torch.tensor([3, 0, 15, 7], device=DEV)
+    kw = dict(rows=4, kv_heads=2, hd=32, page_size=16, fmt=FMT[fmt])
+    hip.cache_write(k, v, ck, cv, ek, ev, slots, **kw)
+    k2, v2 = torch.empty_like(k), torch.empty_like(v)
+    hip.cache_read(ck, cv, ek, ev, slots, k2, v2, **kw)
+    for x, y in ((k, k2), (v, v2)):
+        assert torch.equal(torch.isnan(y).all(-1), ~torch.isfinite(x).all(-1)) and torch.equal(torch.isnan(y).any(-1), ~torch.isfinite(x).all(-1))
+
+
+def test_cache_reads_empty_slots_as_zero_and_takes_strided_rows():
+    hd, HK, page = 32, 2, 16
+    buf = torch.randn((10, 200), generator=gen(2)).half().to(DEV)
+    k, v = buf[:, 8:8 + 64], buf[:, 128:192]
+    planes = new_cache(2, HK, page, hd)
+    kw = dict(rows=10, kv_heads=HK, hd=hd, page_size=page, fmt=hip.CACHE_I8)
+    slots = torch.arange(10, device=DEV) + 9
+    hip.cache_write(k, v, *planes, slots, **kw)
+    dense = new_cache(2, HK, page, hd)
+    hip.cache_write(k.contiguous(), v.contiguous(), *dense, slots, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(planes, dense))
+    out = torch.full((10, 160), 5.0, device=DEV)
+    hip.cache_read(*planes, slots - 9, out[:, :64], out[:, 96:], **kw)
+    back = torch.empty((10, 64), device=DEV), torch.empty((10, 64), device=DEV)
+    hip.cache_read(*planes, slots, *back, **kw)
+    assert torch.equal(out[9:, :64], back[0][:1]) and torch.equal(out[9:, 96:], back[1][:1])
+    assert bool((out[:9, :64] == 0).all()) and bool((out[:9, 96:] == 0).all()) and bool((out[:, 64:96] == 5).all())
+
+
+# ---- attention over the cache --------------------------------------------------------------------------------------------------
+class Memory:
+    """Sequences of the given key counts in a paged cache, garbage (NaN codes, odd exponents) in every slot that belongs to none."""
+
+    def __init__(self, kv_len, kv_heads, hd, page, fmt, seed, spread=1.0):
+        g = gen(seed)
+        held = [-(-n // page) for n in kv_len]
+        pages = sum(held) + 2
+        self.kv_heads, self.hd, self.page, self.fmt = kv_heads, hd, page, fmt
+        self.table = torch.full((len(kv_len), max(1, max(held))), -1, dtype=torch.int32)
+        perm, at = torch.randperm(pages, generator=g).to(torch.int32), 0
+        self.planes = new_cache(pages, kv_heads, page, hd, fill=0x7F)
+        for e in self.planes[2:]:
+            e.fill_(200)
+        slots = []
+        for s, n in enumerate(kv_len):
+            self.table[s, :held[s]] = perm[at:at + held[s]]
+            at += held[s]
+            i = torch.arange(n)
+            slots.append(self.table[s].long()[i // page] * page + i % page)
+        slots = torch.cat(slots).to(DEV)
+        rows = slots.numel()
+        k = torch.randn((rows, kv_heads, hd), generator=g) * torch.exp(spread * torch.randn((rows, kv_heads, 1), generator=g) * 0.3)
+        v = torch.randn((rows, kv_heads, hd), generator=g) * torch.exp(spread * torch.randn((rows, kv_heads, 1), generator=g)) + 0.2
+        if rows:
+            hip.cache_write(k.to(DEV), v.to(DEV), *self.planes, slots, rows=rows, kv_heads=kv_heads, hd=hd, page_size=page, fmt=FMT[fmt])
+        self.slots, self.kv_len = slots, torch.tensor(kv_len, dtype=torch.int32)
+
+    def attend(self, q, q_start, heads, visible=None, scale=None, out=None, **kw):
+        q_start = torch.tensor(q_start, dtype=torch.int32)
+        scale = self.hd ** -0.5 if scale is None else scale
+        out = torch.full_like(q, 3.0) if out is None else out
+        max_q = max(1, int((q_start[1:] - q_start[:-1]).max()))
+        hip.cached_attention(q, out, *self.planes, self.table.to(DEV), self.kv_len.to(DEV), q_start.to(DEV), heads=heads, kv_heads=self.kv_heads,
+                             hd=self.hd, page_size=self.page, fmt=FMT[self.fmt], max_q=max_q, scale=scale,
+                             visible=None if visible is None else visible.to(DEV), **kw)
+        want, tol = R.attend(q, *self.planes, self.table, self.kv_len, q_start, visible, heads, self.kv_heads, self.hd, self.page, self.fmt, scale)
+        rows = ~torch.isnan(want).flatten(1).all(1)
+        return out, want, tol, rows
+
+    def check(self, q, q_start, heads, **kw):
+        out, want, tol, rows = self.attend(q, q_start, heads, **kw)
+        got = out.reshape(q.shape[0], heads, self.hd)
+        within(got[rows.to(DEV)], want[rows], tol[rows])
+        return out, want, rows
+
+
+def queries(rows, heads, hd, dt, seed, size=1.0):
+    return (torch.randn((rows, heads, hd), generator=gen(seed)) * size).to(dt).to(DEV)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("kv_len,q_len,heads,kv_heads,hd,page", [
+    ([1], [1], 1, 1, 8, 16),                               # one key
+    ([130], [1], 6, 6, 64, 1376),                          # one token
+    ([700, 1, 33, 64], [1, 1, 1, 1], 8, 2, 64, 16),        # grouped heads, ragged lengths
+    ([32] * 9, [1] * 9, 8, 8, 32, 32),                     # a temporal module's positions
+    ([7, 40, 17], [2, 5, 3], 4, 4, 24, 16),                # a few tokens each
+    ([300], [3], 16, 1, 128, 32),                          # all heads share one key head
+    ([95, 257], [1, 4], 3, 3, 96, 48),
+    ([90], [2], 2, 2, 48, 16),
+    ([50], [1], 2, 1, 16, 16),
+    ([129], [70], 2, 2, 64, 16),                           # many rows
+    ([65, 200], [33, 129], 2, 1, 32, 64),
+    ([300], [40], 1, 1, 128, 1376),
+    ([140], [37], 2, 2, 96, 16),
+    ([64], [64], 1, 1, 8, 16),
+])
+def test_attention_over_the_cache(kv_len, q_len, heads, kv_heads, hd, page, dt, fmt):
+    m = Memory(kv_len, kv_heads, hd, page, fmt, 11)
+    start = [0]
+    for n in q_len:
+        start.append(start[-1] + n)
+    m.check(queries(start[-1], heads, hd, dt, 12), start, heads)
+
+
+@pytest.mark.parametrize("fmt,dt", [("i8", torch.float16), ("e4m3", torch.bfloat16), ("i8", torch.float32)])
+@pytest.mark.parametrize("q_len", [3, 50, 150])
+def test_attention_sees_only_visible_keys(q_len, fmt, dt):
+    """Causal by frames of seven tokens, rows that see nothing, limits beyond the length; NaN rows among the keys that a row must
+    not see."""
+    kv = q_len + 100
+    m = Memory([kv, 40], 2, 64, 32, fmt, 21)
+    visible = torch.tensor([min(kv, kv - q_len + (i // 7 + 1) * 7) for i in range(q_len)] + [10, 0, -5, 10 ** 9], dtype=torch.int32)
+    q = queries(q_len + 4, 4, 64, dt, 22)
+    out, want, rows = m.check(q, [0, q_len, q_len + 4], 4, visible=visible)
+    assert bool((out[q_len + 1:q_len + 3] == 0).all())
+    last = m.slots[kv - 1]                                  # the first sequence's last key becomes NaN: only rows that see it change
+    bad = torch.full((1, 2, 64), math.nan, device=DEV)
+    hip.cache_write(bad, bad, *m.planes, last[None], rows=1, kv_heads=2, hd=64, page_size=32, fmt=FMT[fmt])
+    again = m.attend(q, [0, q_len, q_len + 4], 4, visible=visible)[0]
+    sees = torch.tensor([n >= kv for n in visible.tolist()])
+    sees[q_len:] = False
+    assert bool(torch.isnan(again[sees.to(DEV)]).all()) and torch.equal(again[~sees.to(DEV)], out[~sees.to(DEV)])
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+@pytest.mark.parametrize("dt", TYPES)
+def test_attention_of_a_visible_nan_row(dt, q_len):
+    m = Memory([50], 1, 32, 16, "e4m3", 31)
+    bad = torch.full((1, 1, 32), math.nan, device=DEV)
+    good = torch.ones((1, 1, 32), device=DEV)
+    hip.cache_write(good, bad, *m.planes, m.slots[20:21], rows=1, kv_heads=1, hd=32, page_size=16, fmt=hip.CACHE_E4M3)
+    q = queries(q_len, 2, 32, dt, 32)
+    out = m.attend(q, [0, q_len], 2)[0]
+    assert bool(torch.isnan(out).all())                     # the value row is NaN, whatever its key
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("q_len,dt", [(1, torch.float16), (1, torch.float32), (5, torch.bfloat16), (40, torch.float16), (40, torch.float32)])
+def test_attention_with_evicted_pages_and_empty_slots(q_len, dt, fmt):
+    m = Memory([200, 90, 0, 31], 2, 64, 16, fmt, 41)
+    m.table[0, 3], m.table[0, 12], m.table[1, 0] = -1, m.planes[0].shape[0], 2 ** 31 - 1      # outside the cache: hidden
+    m.table[3] = -1                                                                            # nothing left
+    m.planes[2].view(-1)[::5] = 0                                                              # empty slots in every page
+    start = [0, q_len, 2 * q_len, 3 * q_len, 4 * q_len]
+    out, want, rows = m.check(queries(4 * q_len, 4, 64, dt, 42), start, 4)
+    assert bool((out[2 * q_len:] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("q_len,dt", [(1, torch.float16), (2, torch.float32), (40, torch.bfloat16), (40, torch.float32)])
+def test_attention_over_rows_of_very_different_sizes(q_len, dt, fmt):
+    """Values whose exponents lie up to thirty octaves apart, zero rows among them, keys of all sizes."""
+    m = Memory([150], 1, 32, 16, fmt, 51)
+    g = gen(52)
+    k = torch.randn((150, 1, 32), generator=g) * torch.exp2(torch.randint(-14, 1, (150, 1, 1), generator=g).float())
+    v = torch.randn((150, 1, 32), generator=g) * torch.exp2(torch.randint(-15, 16, (150, 1, 1), generator=g).float())
+    k[::11], v[::13], v[3] = 0, 0, 0
+    hip.cache_write(k.to(DEV), v.to(DEV), *m.planes, m.slots, rows=150, kv_heads=1, hd=32, page_size=16, fmt=FMT[fmt])
+    m.check(queries(q_len, 1, 32, dt, 53), [0, q_len], 1)
+
+
+@pytest.mark.parametrize("size", [1e-6, 30.0, 3e4])
+@pytest.mark.parametrize("q_len,dt", [(1, torch.float16), (1, torch.bfloat16), (3, torch.float32), (40, torch.bfloat16), (40, torch.float32)])
+def test_attention_with_tiny_and_huge_queries(q_len, dt, size):
+    m = Memory([120], 2, 64, 32, "i8", 61)
+    q = queries(q_len, 2, 64, dt, 62, 1.0)
+    q = (q.float() * size).clamp(-6e4, 6e4).to(dt)
+    m.check(q, [0, q_len], 2, scale=0.125 / size)           # the products, not the operands, set the scores
+    q[0] = 0                                                # a row of zeros weighs all keys alike
+    m.check(q, [0, q_len], 2, scale=0.125 / size)
+
+
+@pytest.mark.parametrize("q_len", [1, 30])
+def test_attention_rows_of_no_sequence_and_strided_rows(q_len):
+    m = Memory([70, 20], 2, 64, 16, "i8", 71)
+    rows = 2 * q_len + 5
+    buf = torch.randn((rows, 3 * 4 * 64), generator=gen(72)).half().to(DEV)
+    out = torch.full((rows, 400), 9.0, dtype=torch.float16, device=DEV)
+    start = [2, 2 + q_len, 2 + 2 * q_len]
+    q = buf[:, 256:512]
+    m.check(q.contiguous().view(rows, 4, 64), start, 4)
+    dense = m.attend(q.contiguous().view(rows, 4, 64), start, 4)[0].reshape(rows, 256)
+    hip.cached_attention(q, out[:, 64:320], *m.planes, m.table.to(DEV), m.kv_len.to(DEV), torch.tensor(start, dtype=torch.int32, device=DEV), heads=4,
+                         kv_heads=2, hd=64, page_size=16, fmt=hip.CACHE_I8, max_q=q_len, scale=0.125)
+    live = slice(2, 2 + 2 * q_len)
+    assert torch.equal(out[live, 64:320], dense[live])
+    assert bool((out[:2] == 9).all()) and bool((out[2 + 2 * q_len:] == 9).all()) and bool((out[:, :64] == 9).all()) and bool((out[:, 320:] == 9).all())
+    # starts beyond the rows are cut to them, lengths beyond the table to it, rows beyond max_q stay as they were
+    start2 = torch.tensor([0, q_len, 10 ** 9], dtype=torch.int32, device=DEV)
+    out.fill_(9.0)
+    hip.cached_attention(q, out[:, 64:320], *m.planes, m.table.to(DEV), torch.tensor([10 ** 9, -3], dtype=torch.int32, device=DEV), start2, heads=4,
+                         kv_heads=2, hd=64, page_size=16, fmt=hip.CACHE_I8, max_q=q_len, scale=0.125)
+    assert bool((out[q_len:2 * q_len, 64:320] == 0).all()) and bool((out[2 * q_len:] == 9).all())
+
+
+@pytest.mark.parametrize("q_len,kv", [(1, 20000), (9, 6000), (64, 5000), (300, 1500)])
+def test_attention_is_the_same_bits_from_run_to_run_and_under_graph_replay(q_len, kv):
+    """The long axis is split over workgroups and joined in a fixed order; the workspace may hold anything."""
+    m = Memory([kv], 2, 64, 64, "i8", 81)
+    q = queries(q_len, 4, 64, torch.float16, 82)
+    table, kv_len, start = m.table.to(DEV), m.kv_len.to(DEV), torch.tensor([0, q_len], dtype=torch.int32, device=DEV)
+    shape = dict(heads=4, kv_heads=2, hd=64, page_size=64, fmt=hip.CACHE_I8, max_q=q_len)
+    n = hip.cached_attention_work(m.planes[0], seqs=1, max_pages=table.shape[1], **shape)
+    work = torch.full((max(n, 16),), 0xFF, dtype=torch.uint8, device=DEV)
+    first, out = torch.empty_like(q), torch.empty_like(q)
+    hip.cached_attention(q, first, *m.planes, table, kv_len, start, scale=0.125, work=work, **shape)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        hip.cached_attention(q, out, *m.planes, table, kv_len, start, scale=0.125, work=work, **shape)
+    for i in range(3):
+        work.fill_(0xFF if i else 0x7F)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first)
+        q.copy_(queries(q_len, 4, 64, torch.float16, 90 + i))
+        hip.cached_attention(q, first, *m.planes, table, kv_len, start, scale=0.125, **shape)
+    if q_len == 1:
+        m.check(q, [0, 1], 4)
+
+
+# ---- norms around a block -------------------------------------------------------------------------------------------------------
+# Statistics: sums of C terms in a tree of at most 40 fp32 additions, the root and the products after it: 48 roundings of 2^-24 of
+# the terms' sizes.
+NORM_ERROR = 48 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("post", ["none", "layer", "rms"])
+@pytest.mark.parametrize("pre", ["none", "layer", "rms"])
+@pytest.mark.parametrize("bt,yt", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.float16)])
+@pytest.mark.parametrize("rows,C,per", [(1, 4, 1), (7, 384, 3), (130, 1024, 64), (5, 1028, 5), (3, 2048, 2), (4, 4096, 1), (3, 5000, 3), (2, 8192, 1), (9, 200, 100)])
+def test_gated_norm(rows, C, per, pre, post, bt, yt):
+    g = gen(rows + C)
+    groups = -(-rows // per)
+    r = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    x, b = (r(rows, C) * 2 + 3).to(DEV), (r(rows, C) + 0.5).to(bt).to(DEV)
+    vec = dict(post_w=1 + 0.2 * r(C), post_b=0.1 * r(C), gate=r(groups, C), pre_w=1 + 0.2 * r(C), pre_b=0.1 * r(C), mod_scale=0.3 * r(groups, C),
+               mod_shift=r(groups, C))
+    if rows == 7:
+        vec = dict.fromkeys(vec)                            # none of them
+    if rows == 9:
+        vec["gate"] = vec["mod_shift"] = vec["post_b"] = vec["pre_b"] = None
+    vec = {n: None if t is None else t.to(DEV) for n, t in vec.items()}
+    x_out, y = torch.full_like(x, math.nan), torch.full((rows, C), math.nan, dtype=yt, device=DEV)
+    kw = dict(rows=rows, C=C, post=NORM[post], pre=NORM[pre], resid_scale=0.8, rows_per_group=per, eps=1e-5, **vec)
+    hip.gated_norm(x, b, x_out, y, **kw)
+    want_x, want_y, size_x, size_y = R.gated_norm(x, b, post, resid_scale=0.8, pre=pre, per=per, eps=1e-5, **vec)
+    within(x_out, want_x, NORM_ERROR * size_x, "x")
+    within(y, want_y, NORM_ERROR * size_y + (0 if yt == torch.float32 else R.half_step(yt)) * (want_y.abs() + NORM_ERROR * size_y), "y")
+    z = x.clone()
+    y2 = torch.empty_like(y)
+    hip.gated_norm(z, b, z, y2, **kw)                       # in place on the stream
+    assert torch.equal(z, x_out) and torch.equal(y2, y)
+
+
+@pytest.mark.parametrize("C", [384, 4100])
+def test_gated_norm_of_the_stream_alone_the_update_alone_and_strided_rows(C):
+    g = gen(C)
+    rows = 6
+    x, b = torch.randn((rows, C + 12), generator=g).to(DEV), torch.randn((rows, 2 * C), generator=g).half().to(DEV)
+    w, gate = torch.randn(C, generator=g).to(DEV), torch.randn((1, C), generator=g).to(DEV)
+    xs, bs = x[:, 4:4 + C], b[:, C:]
+    out, y = torch.zeros((rows, C + 8), device=DEV), torch.zeros((rows, C + 4), dtype=torch.bfloat16, device=DEV)
+    hip.gated_norm(xs, bs, out[:, 8:], y[:, :C], rows=rows, C=C, gate=gate, pre=hip.NORM_RMS, pre_w=w)
+    d_out, d_y = torch.empty((rows, C), device=DEV), torch.empty((rows, C), dtype=torch.bfloat16, device=DEV)
+    hip.gated_norm(xs.contiguous(), bs.contiguous(), d_out, d_y, rows=rows, C=C, gate=gate, pre=hip.NORM_RMS, pre_w=w)
+    assert torch.equal(out[:, 8:], d_out) and torch.equal(y[:, :C], d_y) and bool((out[:, :8] == 0).all()) and bool((y[:, C:] == 0).all())
+    only = torch.empty_like(d_out)
+    hip.gated_norm(xs, bs, only, None, rows=rows, C=C, gate=gate, pre=hip.NORM_NONE)
+    assert torch.equal(only, d_out)
+    y3 = torch.empty_like(d_y)
+    hip.gated_norm(d_out, None, None, y3, rows=rows, C=C, pre=hip.NORM_RMS, pre_w=w)
+    assert torch.equal(y3, d_y)
+
+
+def test_gated_norm_is_the_frameworks_layernorm_on_a_plain_stream():
+    """With a LayerNorm and nothing else it computes what vda_layernorm does, to rounding."""
+    x = torch.randn((50, 1024), generator=gen(1)).to(DEV)
+    w, b = torch.randn(1024, generator=gen(2)).to(DEV), torch.randn(1024, generator=gen(3)).to(DEV)
+    a, y = torch.empty_like(x), torch.empty_like(x)
+    hip.layernorm(x, a, w, b, 50, 1024, 1e-6)
+    hip.gated_norm(x, None, None, y, rows=50, C=1024, pre_w=w, pre_b=b, eps=1e-6)
+    within(y, a.double().cpu(), 2 * NORM_ERROR * (x.abs().double().cpu().amax() * w.abs().double().cpu().amax() + 4))

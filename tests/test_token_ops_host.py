@@ -1,0 +1,218 @@
+"""What the wrappers and the C entries of the rotary, cache, attention and norm operators refuse, before anything is launched, and
+their argument structs against the header."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+import torch
+
+from video_depth_anything import hip
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+EINVAL, ESHAPE = -1, -2
+f16, f32, f64, u8, i32, i64 = torch.float16, torch.float32, torch.float64, torch.uint8, torch.int32, torch.int64
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """The wrappers with the library replaced by a recorder: what reaches the C ABI."""
+    calls = []
+
+    class Recorder:
+        def __getattr__(self, name):
+            return lambda *a: calls.append(name) or 0
+
+    monkeypatch.setattr(hip, "lib", lambda: Recorder())
+    monkeypatch.setattr(hip, "_dev", lambda *ts: None)
+    monkeypatch.setattr(hip, "_current_device", lambda: -1)             # get_device() of a CPU tensor
+    monkeypatch.setattr(hip, "_stream", lambda: None)
+    return calls
+
+
+def test_tensors_of_another_device_or_the_cpu_are_refused(monkeypatch):
+    x = torch.zeros(4, 64, dtype=f16)
+    with pytest.raises(RuntimeError, match="device tensors only"):
+        hip.gated_norm(x.float(), None, None, x, rows=4, C=64)
+    monkeypatch.setattr(hip, "_dev", lambda *ts: None)
+    monkeypatch.setattr(hip, "_current_device", lambda: 0)
+    with pytest.raises(ValueError, match="current device is 0"):
+        hip.gated_norm(x.float(), None, None, x, rows=4, C=64)
+
+
+def test_rotary_wrapper_refusals(recorded):
+    x, pos, freq = torch.zeros(5, 128, dtype=f16), torch.zeros(5, 3, dtype=i32), torch.zeros(16, dtype=f64)
+    kw = dict(rows=5, heads=2, hd=64, sections=(4, 6, 6))
+    hip.rotary_axes(x, x, pos, freq, **kw)
+    hip.rotary_axes(x, x.clone(), pos.float(), freq, **kw)
+    assert len(recorded) == 2
+    for bad, error, match in ((dict(x=x.float()), TypeError, "share"), (dict(pos=pos.long()), TypeError, "int32"), (dict(freq=freq.float()), TypeError, "float64"),
+                              (dict(pos=pos[:4].clone()), ValueError, "pos holds"), (dict(freq=freq[:15].clone()), ValueError, "freq holds"),
+                              (dict(pos=pos.t().contiguous().t()), ValueError, "dense"), (dict(out=x[:4].clone()), ValueError, "out holds"),
+                              (dict(x=torch.zeros(5, 256, dtype=f16)[:, ::2]), ValueError, "not dense"), (dict(rows=6, pos=torch.zeros(6, 3, dtype=i32)), ValueError, "x holds")):
+        args = {**dict(x=x, out=x, pos=pos, freq=freq), **kw, **bad}
+        with pytest.raises(error, match=match):
+            hip.rotary_axes(args.pop("x"), args.pop("out"), args.pop("pos"), args.pop("freq"), **args)
+    assert len(recorded) == 2
+
+
+def planes(pages=3, heads=2, page=16, hd=24):
+    return [torch.zeros(pages, heads, page, hip.cache_row_bytes(hd), dtype=u8) for _ in "kv"] + [torch.zeros(pages, heads, page, dtype=u8) for _ in "kv"]
+
+
+def test_cache_wrapper_refusals(recorded):
+    k, v, slots = torch.zeros(5, 48, dtype=f16), torch.zeros(5, 48, dtype=f16), torch.zeros(5, dtype=i64)
+    pos, freq = torch.zeros(5, 3, dtype=i32), torch.zeros(12, dtype=f64)
+    kw = dict(rows=5, kv_heads=2, hd=24, page_size=16, fmt=hip.CACHE_I8)
+    p = planes()
+    hip.cache_write(k, v, *p, slots, **kw)
+    hip.cache_write(k, v, *p, slots, pos=pos, freq=freq, sections=(4, 4, 4), **kw)
+    hip.cache_read(*p, slots, k, v, **kw)
+    assert recorded == ["vda_cache_write", "vda_cache_write", "vda_cache_read"]
+    for bad, error, match in ((dict(v=v.float()), TypeError, "share"), (dict(slots=slots.int()), TypeError, "int64"), (dict(slots=slots[:4].clone()), ValueError, "slots holds"),
+                              (dict(slots=torch.zeros(10, dtype=i64)[::2]), ValueError, "dense"), (dict(v=v[:4].clone()), ValueError, "v holds"),
+                              (dict(k=torch.zeros(4, 48, dtype=f16)), ValueError, "k holds"), (dict(kv_heads=3), ValueError, "cache plane")):
+        for name in ("write", "read"):
+            a = {**dict(k=k, v=v, slots=slots), **kw, **bad}
+            k_, v_, s_ = a.pop("k"), a.pop("v"), a.pop("slots")
+            with pytest.raises(error, match=match):
+                hip.cache_write(k_, v_, *p, s_, **a) if name == "write" else hip.cache_read(*p, s_, k_, v_, **a)
+    for i in range(4):                                                  # a plane of another type, shape or order
+        for bad in (p[i].to(torch.int8), p[i][:2], p[i].transpose(0, 1).contiguous().transpose(0, 1), p[i][..., :-1].contiguous()):
+            with pytest.raises((TypeError, ValueError), match="cache plane"):
+                hip.cache_write(k, v, *p[:i], bad, *p[i + 1:], slots, **kw)
+    for part in (dict(pos=pos), dict(pos=pos, freq=freq), dict(sections=(4, 4, 4))):
+        with pytest.raises(ValueError, match="come together"):
+            hip.cache_write(k, v, *p, slots, **part, **kw)
+    assert len(recorded) == 3
+
+
+def test_attention_wrapper_refusals(recorded):
+    p = planes()
+    q = torch.zeros(6, 4, 24, dtype=f16)
+    table, kv_len, start, seen = torch.zeros(2, 3, dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(3, dtype=i32), torch.zeros(6, dtype=i32)
+    kw = dict(heads=4, kv_heads=2, hd=24, page_size=16, fmt=hip.CACHE_E4M3, max_q=3, scale=0.2)
+    hip.cached_attention(q, q.clone(), *p, table, kv_len, start, visible=seen, **kw)
+    assert recorded == ["vda_cached_attention_work", "vda_cached_attention"]
+    for bad, error, match in ((dict(out=q.float()), TypeError, "share"), (dict(table=table.long()), TypeError, "int32"), (dict(seen=seen[:5].clone()), ValueError, "visible holds"),
+                              (dict(table=torch.zeros(3, 2, dtype=i32).t()), TypeError, "dense"), (dict(start=start[:2]), ValueError, "belong"),
+                              (dict(kv_len=torch.zeros(3, dtype=i32)), ValueError, "belong"), (dict(out=q[:5].clone()), ValueError, "out holds"),
+                              (dict(q=torch.zeros(6, 4, 48, dtype=f16)[..., ::2]), ValueError, "not dense")):
+        a = {**dict(q=q, out=q.clone(), table=table, kv_len=kv_len, start=start, seen=seen), **bad}
+        with pytest.raises(error, match=match):
+            hip.cached_attention(a["q"], a["out"], *p, a["table"], a["kv_len"], a["start"], visible=a["seen"], **kw)
+
+
+def test_attention_wrapper_refuses_a_small_workspace(recorded, monkeypatch):
+    class Needs:
+        vda_cached_attention_work = staticmethod(lambda *a: 4096)
+        vda_cached_attention = staticmethod(lambda *a: recorded.append("vda_cached_attention") or 0)
+
+    monkeypatch.setattr(hip, "lib", lambda: Needs)
+    p, q = planes(), torch.zeros(1, 4, 24, dtype=f16)
+    one = torch.zeros(1, 3, dtype=i32), torch.zeros(1, dtype=i32), torch.zeros(2, dtype=i32)
+    kw = dict(heads=4, kv_heads=2, hd=24, page_size=16, fmt=hip.CACHE_E4M3, max_q=1, scale=0.2)
+    hip.cached_attention(q, q.clone(), *p, *one, work=torch.zeros(4096, dtype=u8), **kw)
+    with pytest.raises(ValueError, match="work holds 4095"):
+        hip.cached_attention(q, q.clone(), *p, *one, work=torch.zeros(4095, dtype=u8), **kw)
+    assert recorded == ["vda_cached_attention"]
+
+
+def test_norm_wrapper_refusals(recorded):
+    x, b, w = torch.zeros(6, 32), torch.zeros(6, 32, dtype=f16), torch.zeros(32)
+    gate = torch.zeros(3, 32)
+    kw = dict(rows=6, C=32, rows_per_group=2)
+    hip.gated_norm(x, b, x, b.clone(), gate=gate, pre_w=w, **kw)
+    assert recorded == ["vda_gated_norm"]
+    for bad, error, match in ((dict(x=x.half()), TypeError, "x is fp32"), (dict(gate=gate[:2].clone()), ValueError, "gate holds"), (dict(gate=gate.half()), TypeError, "gate is fp32"),
+                              (dict(gate=torch.zeros(3, 64)[:, ::2]), ValueError, "dense"), (dict(pre_w=w[:31].clone()), ValueError, "pre_w holds"),
+                              (dict(b=b.to(i32)), TypeError, "b and y"), (dict(y=b[:5].clone()), ValueError, "y holds"), (dict(rows_per_group=0), ValueError, "positive"),
+                              (dict(x_out=x[:5].clone()), ValueError, "x_out holds")):
+        a = {**dict(x=x, b=b, x_out=x, y=b.clone(), gate=gate, pre_w=w), **kw, **bad}
+        with pytest.raises(error, match=match):
+            hip.gated_norm(a.pop("x"), a.pop("b"), a.pop("x_out"), a.pop("y"), **a)
+    assert len(recorded) == 1
+
+
+# ---- the C entries: every call below is refused before a launch (the pointers are never followed) -----------------------------------
+A = 1 << 20                                                             # some 16-byte aligned address
+
+
+def test_c_rotary_refusals():
+    f = hip.lib().vda_rotary_axes
+    good = dict(x=A, out=2 * A, pos=A, freq=A, rows=4, heads=2, hd=64, ldx=128, ldo=128, n_t=8, n_h=12, n_w=12, pairing=0, pos_float=0, dtype=hip.T_F16, stream=None)
+    for bad, rc in ((dict(x=None), EINVAL), (dict(out=None), EINVAL), (dict(pos=None), EINVAL), (dict(freq=None), EINVAL), (dict(rows=0), EINVAL), (dict(heads=0), EINVAL),
+                    (dict(dtype=0), EINVAL), (dict(dtype=7), EINVAL), (dict(pairing=2), EINVAL), (dict(n_t=-4, n_h=24), EINVAL), (dict(n_t=9), ESHAPE),
+                    (dict(n_t=12), ESHAPE), (dict(n_t=0, n_h=0, n_w=0), ESHAPE), (dict(hd=60, n_t=0), ESHAPE), (dict(hd=264, ldx=528, ldo=528), ESHAPE),
+                    (dict(ldx=120), ESHAPE), (dict(ldo=64), ESHAPE), (dict(x=A + 8), ESHAPE), (dict(ldx=129), ESHAPE), (dict(x=A + 4, out=A + 4), ESHAPE),
+                    (dict(out=A, ldo=256), EINVAL), (dict(dtype=hip.T_F32, x=A + 8), ESHAPE), (dict(rows=1 << 50), ESHAPE)):
+        assert f(*{**good, **bad}.values()) == rc, bad
+
+
+def desc(**bad):
+    return hip.CacheDesc(*{**dict(k=A, v=A, k_exp=A, v_exp=A, pages=4, page_size=32, kv_heads=2, hd=64, format=0), **bad}.values())
+
+
+BAD_CACHES = [(dict(k=None), EINVAL), (dict(v=None), EINVAL), (dict(k_exp=None), EINVAL), (dict(v_exp=None), EINVAL), (dict(pages=0), EINVAL), (dict(page_size=-16), EINVAL),
+              (dict(kv_heads=0), EINVAL), (dict(hd=0), EINVAL), (dict(format=2), EINVAL), (dict(hd=20), ESHAPE), (dict(hd=136), ESHAPE), (dict(page_size=24), ESHAPE),
+              (dict(k=A + 8), ESHAPE), (dict(v_exp=A + 1), ESHAPE), (dict(pages=1 << 27), ESHAPE)]
+
+
+def test_c_cache_refusals():
+    w, r = hip.lib().vda_cache_write, hip.lib().vda_cache_read
+    good = dict(k=A, v=A, slots=A, rows=4, ldk=128, ldv=128, dtype=hip.T_BF16, pos=A, freq=A, n_t=8, n_h=12, n_w=12, pairing=0, pos_float=0, stream=None)
+    read = lambda a: (a["slots"], a["k"], a["v"], a["rows"], a["ldk"], a["ldv"], a["dtype"], None)  # noqa: E731
+    for bad, rc in BAD_CACHES:
+        assert w(ctypes.byref(desc(**bad)), *good.values()) == rc and r(ctypes.byref(desc(**bad)), *read(good)) == rc, bad
+    for bad, rc in ((dict(k=None), EINVAL), (dict(v=None), EINVAL), (dict(slots=None), EINVAL), (dict(rows=0), EINVAL), (dict(dtype=0), EINVAL), (dict(ldk=120), ESHAPE),
+                    (dict(ldv=127), ESHAPE), (dict(ldv=129), ESHAPE), (dict(k=A + 8), ESHAPE), (dict(rows=1 << 50), ESHAPE)):
+        a = {**good, **bad}
+        assert w(ctypes.byref(desc()), *a.values()) == rc and r(ctypes.byref(desc()), *read(a)) == rc, bad
+    for bad, rc in ((dict(pos=None), EINVAL), (dict(freq=None), EINVAL), (dict(pairing=5), EINVAL), (dict(n_t=9), ESHAPE), (dict(n_t=12), ESHAPE), (dict(n_w=-4), EINVAL)):
+        assert w(ctypes.byref(desc()), *{**good, **bad}.values()) == rc, bad
+    assert w(None, *good.values()) == EINVAL and r(None, *read(good)) == EINVAL
+
+
+def attention_args(**bad):
+    return hip.CachedAttentionArgs(*{**dict(q=A, out=A, page_table=A, kv_len=A, q_start=A, visible=None, work=A, work_bytes=1 << 40, rows=8, ldq=256, ldo=256, seqs=2,
+                                            max_pages=4, max_q=4, heads=4, dtype=hip.T_F16, scale=0.1), **bad}.values())
+
+
+def test_c_attention_refusals():
+    f, n = hip.lib().vda_cached_attention, hip.lib().vda_cached_attention_work
+    for bad, rc in BAD_CACHES:
+        assert f(ctypes.byref(desc(**bad)), ctypes.byref(attention_args()), None) == rc and n(ctypes.byref(desc(**bad)), 2, 4, 4, 4) == rc, bad
+    for bad, rc in ((dict(q=None), EINVAL), (dict(out=None), EINVAL), (dict(page_table=None), EINVAL), (dict(kv_len=None), EINVAL), (dict(q_start=None), EINVAL),
+                    (dict(rows=0), EINVAL), (dict(seqs=0), EINVAL), (dict(max_pages=0), EINVAL), (dict(max_q=0), EINVAL), (dict(heads=0), EINVAL), (dict(dtype=0), EINVAL),
+                    (dict(heads=3), ESHAPE), (dict(ldq=255), ESHAPE), (dict(ldo=248), ESHAPE), (dict(ldq=257), ESHAPE), (dict(q=A + 8), ESHAPE), (dict(out=A + 2), ESHAPE),
+                    (dict(max_pages=1 << 27), ESHAPE)):
+        assert f(ctypes.byref(desc()), ctypes.byref(attention_args(**bad)), None) == rc, bad
+    assert f(ctypes.byref(desc()), None, None) == EINVAL and f(None, ctypes.byref(attention_args()), None) == EINVAL
+    for bad, rc in (((0, 4, 4, 4), EINVAL), ((2, 0, 4, 4), EINVAL), ((2, 4, 0, 4), EINVAL), ((2, 4, 4, 0), EINVAL), ((2, 4, 4, 3), ESHAPE), ((2, 1 << 27, 4, 4), ESHAPE)):
+        assert n(ctypes.byref(desc()), *bad) == rc, bad
+
+
+def test_c_norm_refusals():
+    f = hip.lib().vda_gated_norm
+    good = dict(x=A, b=A, x_out=A, y=A, post_w=A, post_b=A, gate=A, pre_w=A, pre_b=A, mod_scale=A, mod_shift=A, rows=4, ldx=64, ldb=64, ldxo=64, ldy=64, C=64,
+                rows_per_group=2, post=1, pre=2, b_type=hip.T_F16, y_type=hip.T_BF16, resid_scale=1.0, eps=1e-6)
+    alone = dict(b=None, x_out=None, post=0, post_w=None, post_b=None, gate=None)
+    for bad, rc in ((dict(x=None), EINVAL), (dict(rows=0), EINVAL), (dict(C=0), EINVAL), (dict(rows_per_group=0), EINVAL), (dict(post=3), EINVAL), (dict(pre=-1), EINVAL),
+                    (dict(b=None), EINVAL), (dict(x_out=None), EINVAL), (dict(alone, y=None), EINVAL), (dict(alone, gate=A), EINVAL), (dict(alone, post=2), EINVAL),
+                    (dict(y=None), EINVAL), (dict(y=None, pre=0, mod_scale=None, mod_shift=None, pre_w=None), EINVAL), (dict(b_type=0), EINVAL), (dict(y_type=9), EINVAL),
+                    (dict(C=62), ESHAPE), (dict(C=8196, ldx=8196, ldb=8196, ldxo=8196, ldy=8196), ESHAPE), (dict(ldx=60), ESHAPE), (dict(ldb=63), ESHAPE),
+                    (dict(ldy=66), ESHAPE), (dict(x=A + 4), ESHAPE), (dict(b=A + 4), ESHAPE), (dict(gate=A + 8), ESHAPE), (dict(ldxo=68), EINVAL), (dict(rows=1 << 50), ESHAPE)):
+        assert f(ctypes.byref(hip.GatedNormArgs(*{**good, **bad}.values())), None) == rc, bad
+    assert f(None, None) == EINVAL
+
+
+def test_argument_structs_match_the_header(tmp_path):
+    fields = [(n, f) for s, n in ((hip.CacheDesc, "VdaTokenCache"), (hip.CachedAttentionArgs, "VdaCachedAttentionArgs"), (hip.GatedNormArgs, "VdaGatedNormArgs"))
+              for f in [x[0] for x in s._fields_]]
+    body = "".join('printf("%%zu\\n", offsetof(%s, %s));' % x for x in fields)
+    sizes = "".join('printf("%%zu\\n", sizeof(%s));' % n for n in ("VdaTokenCache", "VdaCachedAttentionArgs", "VdaGatedNormArgs"))
+    (tmp_path / "t.c").write_text('#include <stdio.h>\n#include <stddef.h>\n#include "vda_hip.h"\nint main(void) {' + body + sizes + "return 0; }\n")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(tmp_path / "t.c"), "-o", str(tmp_path / "t")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.split()]
+    of = {"VdaTokenCache": hip.CacheDesc, "VdaCachedAttentionArgs": hip.CachedAttentionArgs, "VdaGatedNormArgs": hip.GatedNormArgs}
+    assert got == [getattr(of[n], f).offset for n, f in fields] + [ctypes.sizeof(s) for s in of.values()]

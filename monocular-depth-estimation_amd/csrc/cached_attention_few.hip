@@ -1,0 +1,367 @@
+// Attention over the token cache for few query rows per key head (single tokens, a temporal module's positions).
+//
+// Memory bound: every cached byte is read once and meets at most 16 query rows, which all sit in one 16-wide matrix instruction.  A
+// wave works on its own 32 keys at a time.  Scores are S^T = K Q^T (mfma 16x16x32 on IEEE halves): the keys' codes go from global
+// memory to registers in the operand's order (the order of channels within a row is free as long as q uses the same), become
+// halves there, and the exponent of a key multiplies its four scores.  A lane then holds one query's scores of keys
+// 4g .. 4g+3 (g = lane / 16) of two blocks of 16, which, exponentiated, is the B operand of O^T = V^T P^T if the 8 keys of lane group g
+// are taken in that order.  V^T needs 8 keys of one channel per lane: the codes pass through LDS, whose transposed
+// 16-bit read delivers pairs of channels, even and odd channels becoming two operands.  A value's exponent multiplies its
+// probability (relative to the largest exponent so far), so codes are never scaled.  The loads of the next 32 keys are in
+// flight while these are multiplied.
+#include "cached_attention.h"
+
+namespace {
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// byte offset of (key, byte column) in a wave's V tile: 32-byte segments of a row are permuted so that the eight rows which half a
+// wave reads together start in different banks
+template <int HDP>
+__device__ __forceinline__ int vtile(int key, int col) {
+    const int swz = HDP == 64 ? ((key >> 2) & 1) << 5 : HDP == 128 ? ((key >> 1) & 3) << 5 : 0;
+    return key * HDP + (col ^ swz);
+}
+
+template <int HDP> struct Step {
+    u32x4 k[2][HDP >= 64 ? HDP / 64 : 1];         // 64 channels of a key: 16 bytes per lane
+    u32x2 k8[2];                                  // 32 channels of a key: 8 bytes per lane (HDP 32 and 96)
+    u32x4 v[HDP / 32];
+    unsigned ek[2], ev[2];
+};
+
+// W waves share a (sequence, key head, row block, split) item, each with a part of its keys; W = 1: a wave per item.
+template <typename T, int HDP, int FMT, int W>
+__global__ __launch_bounds__(256) void attend_few_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int items) {
+    constexpr int NP = Pieces<T>::n, C64 = HDP / 64, TAIL32 = (HDP / 32) & 1, CB = HDP / 32;
+    constexpr int JOIN = W == 1 ? 0 : W * (HDP * 16 + 32) * 4, TILES = 4 * 32 * HDP;
+    __shared__ __attribute__((aligned(16))) char smem[JOIN > TILES ? JOIN : TILES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g = lane >> 4;
+    int id = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    if (W == 1 && id >= items) return;
+    const int split = id % j.splits;
+    const int item = id / j.splits;
+    const int kvh = item % j.kv_heads, t0 = item / j.kv_heads, rb = t0 % j.row_blocks, s = t0 / j.row_blocks;
+    const Span sp = span_of(j, s, max_q);
+    const int rho = rb * 16 + c16, n_rho = sp.nq * j.group;
+    if (rb * 16 >= n_rho) return;                                   // the whole workgroup
+    const int token = rho / j.group, head = kvh * j.group + (rho - token * j.group);
+    const bool live = rho < n_rho;
+    const long row = sp.q0 + (live ? token : 0);
+    int limit = live ? sp.n : 0;
+    if (j.visible && live) limit = max(0, min(limit, j.visible[row]));
+
+    // the keys that any row of the block sees, dealt to the splits and waves in runs of whole steps
+    int most = limit;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o));
+    most = __builtin_amdgcn_readfirstlane(most);
+    const int parts = j.splits * W, steps = (most + 31) / 32, per = (steps + parts - 1) / parts;
+    const int part = split * W + (W == 1 ? 0 : wave);
+    const int k_begin = min(part * per, steps) * 32, k_end = min(k_begin + per * 32, most);
+
+    f16x8 qf[2 * C64 + TAIL32][NP];
+    float c_row;
+    {
+        float f[2 * C64 + TAIL32][8], amax = 0.f;
+        const T* qr = q + row * j.ldq + (long)head * j.hd;
+#pragma unroll
+        for (int i = 0; i < 2 * C64 + TAIL32; ++i) {
+            const int e = i < 2 * C64 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 64 * C64 + 8 * g;
+            query8<T>(qr + e, live && e < j.hd, f[i]);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) amax = fmaxf(amax, fabsf(f[i][x]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 16));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int shift = query_shift(amax);
+#pragma unroll
+        for (int i = 0; i < 2 * C64 + TAIL32; ++i) query_pieces<NP>(f[i], shift, qf[i]);
+        c_row = __builtin_amdgcn_ldexpf(j.scale_log2e, -shift);
+    }
+
+    // this lane's part of a V tile: it copies 16 bytes of HDP / 32 keys
+    char* vt = smem + wave * (32 * HDP);
+    int v_key[CB], v_col[CB], v_lds[CB];
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        const int idx = i * 64 + lane;
+        v_key[i] = idx / (HDP / 16);
+        const int col = (idx % (HDP / 16)) * 16;
+        v_col[i] = min(col, j.row_bytes - 16);
+        v_lds[i] = vtile<HDP>(v_key[i], col);
+    }
+    const int k_off8 = min(64 * C64 + 8 * g, j.row_bytes - 8);
+
+    // the pages of a step's two blocks of 16 keys (a page holds a multiple of 16 slots); a block without one reads as empty slots
+    int pi = k_begin / j.page_size, off = k_begin - pi * j.page_size;
+    const int* table = j.page_table + (long)s * j.max_pages;
+    auto block_row = [&](int key) -> long {
+        long r = -1;
+        if (key < k_end) {
+            const int page = table[pi];
+            if (page >= 0 && page < j.pages) r = ((long)page * j.kv_heads + kvh) * j.page_size + off;
+        }
+        off += 16;
+        if (off >= j.page_size) { off = 0; ++pi; }
+        return r;
+    };
+    auto fetch = [&](Step<HDP>& st, int k0) {
+        long r[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            r[b] = block_row(k0 + 16 * b);
+            const bool any = r[b] >= 0;
+            if (!any) r[b] = 0;                                     // slot 0 exists: its bytes are read and not used
+            const uint8_t* kr = j.k + (r[b] + c16) * j.row_bytes;
+#pragma unroll
+            for (int i = 0; i < C64; ++i) st.k[b][i] = *reinterpret_cast<const u32x4*>(kr + min(64 * i + 16 * g, j.row_bytes - 16));
+            if (TAIL32) st.k8[b] = *reinterpret_cast<const u32x2*>(kr + k_off8);
+            st.ek[b] = *reinterpret_cast<const unsigned*>(j.k_exp + r[b] + 4 * g);
+            st.ev[b] = *reinterpret_cast<const unsigned*>(j.v_exp + r[b] + 4 * g);
+            if (!any) st.ek[b] = 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < CB; ++i)
+            st.v[i] = *reinterpret_cast<const u32x4*>(j.v + ((v_key[i] < 16 ? r[0] : r[1]) + (v_key[i] & 15)) * j.row_bytes + v_col[i]);
+    };
+
+    f32x4 o[CB][2];
+#pragma unroll
+    for (int i = 0; i < CB; ++i) { o[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; o[i][1] = o[i][0]; }
+    float m_run = LOWEST, l_run = 0.f;
+    int v_ref = 1;                                                  // largest exponent byte of V so far, the same in every lane
+
+    Step<HDP> now, next;
+    if (k_begin < k_end) fetch(now, k_begin);
+    for (int k0 = k_begin; k0 < k_end; k0 += 32) {
+        if (k0 + 32 < k_end) fetch(next, k0 + 32);
+        // V codes to LDS (in the order of the keys); the wave alone reads them, LDS operations of a wave stay in order
+#pragma unroll
+        for (int i = 0; i < CB; ++i) *reinterpret_cast<u32x4*>(vt + v_lds[i]) = now.v[i];
+        asm volatile("" ::: "memory");
+
+        float sc[2][4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < C64; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f16x8 kf = codes8<FMT>(u32x2{now.k[b][i][2 * h], now.k[b][i][2 * h + 1]});
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) a = mfma16(kf, qf[2 * i + h][p], a);
+                }
+            if (TAIL32) {
+                const f16x8 kf = codes8<FMT>(now.k8[b]);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) a = mfma16(kf, qf[2 * C64][p], a);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[b][i] = a[i] * (c_row * power_of_byte(byte_of(now.ek[b], i)));
+        }
+        // what is not seen: keys beyond the row's limit, empty slots; what is seen and not a number: rows with exponent 255
+        unsigned keep[2] = {0xffffffffu, 0xffffffffu};
+        const unsigned odd = zero_bytes(now.ek[0]) | zero_bytes(now.ek[1]) | zero_bytes(~now.ek[0]) | zero_bytes(~now.ek[1]) | zero_bytes(~now.ev[0]) | zero_bytes(~now.ev[1]);
+        if (__builtin_amdgcn_ballot_w64(odd != 0 || k0 + 32 > limit || k0 + 32 > k_end) != 0) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                keep[b] = 0u;
+                unsigned ev = 0u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = k0 + 16 * b + 4 * g + i, e = byte_of(now.ek[b], i), w = byte_of(now.ev[b], i);
+                    const bool nan = e == 255 || w == 255;
+                    if (key >= k_end || e == 0) {
+                        sc[b][i] = -INFINITY;
+                    } else if (nan) {
+                        sc[b][i] = key < limit ? __builtin_nanf("") : -INFINITY;
+                    } else {
+                        keep[b] |= 255u << (8 * i);
+                        ev |= (unsigned)w << (8 * i);
+                        if (key >= limit) sc[b][i] = -INFINITY;
+                    }
+                }
+                now.ev[b] = ev;
+            }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        int ve[2][4], top = 0;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { ve[b][i] = byte_of(now.ev[b], i); top = max(top, ve[b][i]); }
+        if (__builtin_amdgcn_ballot_w64(mx > m_run + DEFER || top > v_ref) != 0) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            top = max(top, __shfl_xor(top, 16));
+            top = max(top, __shfl_xor(top, 32));
+            const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            const int ref = max(v_ref, top);
+            const float beta = __builtin_amdgcn_ldexpf(alpha, v_ref - ref);
+            l_run *= alpha;
+#pragma unroll
+            for (int i = 0; i < CB; ++i) { o[i][0] *= beta; o[i][1] *= beta; }
+            m_run = m_new;
+            v_ref = ref;
+        }
+        f16x8 pf[NP];
+        float sum = 0.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(sc[b][i] - m_run);
+                sum += p;
+                const float w = __builtin_amdgcn_ldexpf(p, ve[b][i] - v_ref + P_SHIFT);
+                const f16 hi = (f16)w;
+                pf[0][4 * b + i] = hi;
+                if (NP == 2) pf[NP - 1][4 * b + i] = (f16)(w - (float)hi);
+            }
+        l_run += sum;
+
+        // (a hidden key's value codes may be anything, e4m3's NaN too: 0 times them has to be 0)
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            const int q4 = c16 >> 2, p4 = c16 & 3;
+            const u32x2 r0 = __builtin_bit_cast(u32x2, read_tr<f16>(vt + vtile<HDP>(4 * g + q4, 32 * i + 8 * p4)));
+            const u32x2 r1 = __builtin_bit_cast(u32x2, read_tr<f16>(vt + vtile<HDP>(16 + 4 * g + q4, 32 * i + 8 * p4)));
+#pragma unroll
+            for (int par = 0; par < 2; ++par) {
+                const unsigned sel = par ? 0x07050301u : 0x06040200u;
+                const u32x2 w = {__builtin_amdgcn_perm(r0[1], r0[0], sel) & keep[0], __builtin_amdgcn_perm(r1[1], r1[0], sel) & keep[1]};
+                const f16x8 vf = codes8<FMT>(w);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) o[i][par] = mfma16(vf, pf[p], o[i][par]);
+            }
+        }
+        now = next;
+    }
+
+    // lane (c16, g) holds channels 32 i + 8 g + 0..7 of query c16, even ones in o[i][0], odd ones in o[i][1]
+    l_run += __shfl_xor(l_run, 16);
+    l_run += __shfl_xor(l_run, 32);
+#pragma unroll
+    for (int i = 0; i < CB; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            o[i][0][x] = __builtin_amdgcn_ldexpf(o[i][0][x], v_ref - 127 - P_SHIFT);
+            o[i][1][x] = __builtin_amdgcn_ldexpf(o[i][1][x], v_ref - 127 - P_SHIFT);
+        }
+    if (W > 1) {        // join the waves' parts: [wave][16 rows][HDP] outputs, then [wave][16] maxima and sums
+        __syncthreads();                                            // the V tiles are done with
+        float* jo = reinterpret_cast<float*>(smem);
+        float* jm = jo + W * 16 * HDP;
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            float* p = jo + (wave * 16 + c16) * HDP + 32 * i + 8 * g;
+            *reinterpret_cast<f32x4*>(p) = f32x4{o[i][0][0], o[i][1][0], o[i][0][1], o[i][1][1]};
+            *reinterpret_cast<f32x4*>(p + 4) = f32x4{o[i][0][2], o[i][1][2], o[i][0][3], o[i][1][3]};
+        }
+        if (g == 0) { jm[wave * 16 + c16] = m_run; jm[W * 16 + wave * 16 + c16] = l_run; }
+        __syncthreads();
+        if (wave != 0) return;
+        float m = LOWEST;
+#pragma unroll
+        for (int w = 0; w < W; ++w) m = fmaxf(m, jm[w * 16 + c16]);
+        l_run = 0.f;
+#pragma unroll
+        for (int i = 0; i < CB; ++i) { o[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; o[i][1] = o[i][0]; }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float a = __builtin_amdgcn_exp2f(jm[w * 16 + c16] - m);
+            l_run += a * jm[W * 16 + w * 16 + c16];
+#pragma unroll
+            for (int i = 0; i < CB; ++i) {
+                const float* p = jo + (w * 16 + c16) * HDP + 32 * i + 8 * g;
+                const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+                o[i][0] += a * f32x4{x[0], x[2], y[0], y[2]};
+                o[i][1] += a * f32x4{x[1], x[3], y[1], y[3]};
+            }
+        }
+        m_run = m;
+    }
+    if (!live) return;
+    if (j.splits > 1) {
+        float* p = j.part + ((long)item * j.splits + split) * (16 * (HDP + 2));
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            float* d = p + c16 * HDP + 32 * i + 8 * g;
+            *reinterpret_cast<f32x4*>(d) = f32x4{o[i][0][0], o[i][1][0], o[i][0][1], o[i][1][1]};
+            *reinterpret_cast<f32x4*>(d + 4) = f32x4{o[i][0][2], o[i][1][2], o[i][0][3], o[i][1][3]};
+        }
+        if (g == 0) { p[16 * HDP + c16] = m_run; p[16 * HDP + 16 + c16] = l_run; }
+        return;
+    }
+    const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+    T* orow = out + row * j.ldo + (long)head * j.hd;
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        const int d = 32 * i + 8 * g;
+        if (d >= j.hd) continue;
+        typename Vec<T>::v8 r;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) { r[2 * x] = (T)(o[i][0][x] * inv); r[2 * x + 1] = (T)(o[i][1][x] * inv); }
+        *reinterpret_cast<typename Vec<T>::v8*>(orow + d) = r;
+    }
+}
+
+// The parts of a row block joined in their order: out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.  One workgroup per item.
+template <typename T>
+__global__ __launch_bounds__(256) void attend_join_kernel(T* __restrict__ out, AttendJob j, int max_q, int block_rows, int hdp) {
+    const int item = blockIdx.x, kvh = item % j.kv_heads, t0 = item / j.kv_heads, rb = t0 % j.row_blocks, s = t0 / j.row_blocks;
+    const Span sp = span_of(j, s, max_q);
+    const int rows = min(block_rows, sp.nq * j.group - rb * block_rows), quads = j.hd / 4;
+    const long stride = (long)block_rows * (hdp + 2);
+    const float* p = j.part + (long)item * j.splits * stride;
+    for (int i = threadIdx.x; i < rows * quads; i += 256) {
+        const int r = i / quads, d = (i - r * quads) * 4;
+        float m = LOWEST, l = 0.f;
+        for (int x = 0; x < j.splits; ++x) m = fmaxf(m, p[x * stride + block_rows * hdp + r]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < j.splits; ++x) {
+            const float a = __builtin_amdgcn_exp2f(p[x * stride + block_rows * hdp + r] - m);
+            l += a * p[x * stride + block_rows * hdp + block_rows + r];
+            o += a * *reinterpret_cast<const f32x4*>(p + x * stride + r * hdp + d);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int rho = rb * block_rows + r, token = rho / j.group;
+        const typename Vec<T>::v4 y = {(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+        *reinterpret_cast<typename Vec<T>::v4*>(out + (sp.q0 + token) * j.ldo + (long)(kvh * j.group + rho - token * j.group) * j.hd + d) = y;
+    }
+}
+
+template <typename T>
+int few(const AttendJob& j, const T* q, T* out, int format, int max_q, int waves, hipStream_t st) {
+    const int items = j.seqs * j.kv_heads * j.row_blocks * j.splits;
+    const int grid = waves == 1 ? (items + 3) / 4 : items;
+#define VDA_F3(H, F, W) hipLaunchKernelGGL((attend_few_kernel<T, H, F, W>), dim3(grid), dim3(256), 0, st, q, out, j, max_q, items)
+#define VDA_F2(H, F) do { if (waves == 1) VDA_F3(H, F, 1); else VDA_F3(H, F, 4); } while (0)
+#define VDA_F(H) do { if (format == VDA_CACHE_I8) VDA_F2(H, VDA_CACHE_I8); else VDA_F2(H, VDA_CACHE_E4M3); } while (0)
+    if (j.hd <= 32) VDA_F(32);
+    else if (j.hd <= 64) VDA_F(64);
+    else if (j.hd <= 96) VDA_F(96);
+    else VDA_F(128);
+#undef VDA_F
+#undef VDA_F2
+#undef VDA_F3
+    return hip_rc(hipGetLastError());
+}
+
+}  // namespace
+
+int attend_few(const AttendJob& j, const void* q, void* out, int dtype, int format, int max_q, int waves, hipStream_t st) {
+    if (dtype == VDA_T_BF16) return few(j, (const bf16*)q, (bf16*)out, format, max_q, waves, st);
+    if (dtype == VDA_T_F16) return few(j, (const f16*)q, (f16*)out, format, max_q, waves, st);
+    return few(j, (const float*)q, (float*)out, format, max_q, waves, st);
+}
+
+int attend_join(const AttendJob& j, void* out, int dtype, int max_q, int block_rows, int hd_pad, hipStream_t st) {
+    const dim3 grid(j.seqs * j.kv_heads * j.row_blocks);
+    if (dtype == VDA_T_BF16) hipLaunchKernelGGL((attend_join_kernel<bf16>), grid, dim3(256), 0, st, (bf16*)out, j, max_q, block_rows, hd_pad);
+    else if (dtype == VDA_T_F16) hipLaunchKernelGGL((attend_join_kernel<f16>), grid, dim3(256), 0, st, (f16*)out, j, max_q, block_rows, hd_pad);
+    else hipLaunchKernelGGL((attend_join_kernel<float>), grid, dim3(256), 0, st, (float*)out, j, max_q, block_rows, hd_pad);
+    return hip_rc(hipGetLastError());
+}

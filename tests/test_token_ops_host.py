@@ -192,6 +192,16 @@ def test_c_attention_refusals():
         assert n(ctypes.byref(desc()), *bad) == rc, bad
 
 
+def test_c_attention_refuses_a_missing_or_small_workspace():
+    """Sizes whose long axis is split need the workspace."""
+    f, n = hip.lib().vda_cached_attention, hip.lib().vda_cached_attention_work
+    d = desc(pages=2000, page_size=64)
+    need = n(ctypes.byref(d), 1, 1000, 1, 4)
+    assert need > 0
+    for bad, rc in ((dict(work=None), EINVAL), (dict(work_bytes=need - 1), ESHAPE), (dict(work=A + 4), ESHAPE)):
+        assert f(ctypes.byref(d), ctypes.byref(attention_args(seqs=1, max_pages=1000, max_q=1, **bad)), None) == rc, bad
+
+
 def test_c_norm_refusals():
     f = hip.lib().vda_gated_norm
     good = dict(x=A, b=A, x_out=A, y=A, post_w=A, post_b=A, gate=A, pre_w=A, pre_b=A, mod_scale=A, mod_shift=A, rows=4, ldx=64, ldb=64, ldxo=64, ldy=64, C=64,

@@ -94,4 +94,5 @@ __device__ __forceinline__ unsigned zero_bytes(unsigned w) { return (w - 0x01010
 __device__ __forceinline__ float power_of_byte(int byte) { return __uint_as_float((unsigned)byte << 23); }      // 2^(byte - 127), 1 <= byte <= 254
 
 int attend_few(const AttendJob& j, const void* q, void* out, int dtype, int format, int max_q, int waves, hipStream_t st);
+int attend_many(const AttendJob& j, const void* q, void* out, int dtype, int format, int max_q, hipStream_t st);
 int attend_join(const AttendJob& j, void* out, int dtype, int max_q, int block_rows, int hd_pad, hipStream_t st);

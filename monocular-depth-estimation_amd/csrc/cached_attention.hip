@@ -9,20 +9,31 @@ struct Plan {
     long work;
 };
 
-// Enough waves in flight to draw the full memory bandwidth: a few thousand.  Where the (sequence, key head, row block) items alone
+// Up to 32 rows per key head: the kernel whose waves hold 16 rows each and read the cache straight into registers.  It wants
+// enough waves in flight to draw the full memory bandwidth, a few thousand: where the (sequence, key head, row block) items alone
 // are fewer, four waves share an item and the key axis is split over workgroups, down to 128 keys for each wave.
+// More rows: the kernel whose workgroups of 128 rows share decoded tiles; the key axis is split, down to 512 keys, until the
+// workgroups that a CU holds at once (three, two for wide heads) are there.
+constexpr int FEW_ROWS = 32;
 int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int heads, Plan* p) {
     if (const int rc = cache_check(c)) return rc;
     if (seqs <= 0 || max_pages <= 0 || max_q <= 0 || heads <= 0) return VDA_EINVAL;
     if (heads % c->kv_heads != 0 || (long)max_pages * c->page_size > 0x7fffffffL) return VDA_ESHAPE;
     const long rows = (long)max_q * (heads / c->kv_heads), keys = (long)max_pages * c->page_size;
-    p->block_rows = 16;
+    const bool few = rows <= FEW_ROWS;
+    p->block_rows = few ? 16 : 128;
     p->hd_pad = (c->hd + 31) & ~31;
-    const long blocks = (rows + 15) / 16, items = blocks * seqs * c->kv_heads;
+    const long blocks = (rows + p->block_rows - 1) / p->block_rows, items = blocks * seqs * c->kv_heads;
     if (rows > 0x7fffffffL || items > 0x3fffffffL) return VDA_ESHAPE;
-    const long target = 4096;
-    p->waves = items >= target || keys <= 64 ? 1 : 4;
-    long splits = p->waves == 1 ? 1 : target / (items * 4);
+    long splits;
+    if (few) {
+        const long target = 4096;
+        p->waves = items >= target || keys <= 64 ? 1 : 4;
+        splits = p->waves == 1 ? 1 : target / (items * 4);
+    } else {
+        p->waves = 0;
+        splits = 256 * (c->hd <= 64 ? 3 : 2) / items;
+    }
     splits = splits > keys / 512 ? keys / 512 : splits;
     p->splits = (int)(splits < 1 ? 1 : splits);
     p->row_blocks = (int)blocks;
@@ -55,6 +66,8 @@ extern "C" int vda_cached_attention(const VdaTokenCache* cache, const VdaCachedA
                       (float*)a->work, a->rows, a->ldq, a->ldo, cache->pages, cache->page_size, cache->kv_heads, cache->hd, cache_row_bytes(cache->hd),
                       a->max_pages, a->heads / cache->kv_heads, a->seqs, p.row_blocks, p.splits, a->scale * 1.4426950408889634f};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (const int rc = attend_few(j, a->q, a->out, a->dtype, cache->format, a->max_q, p.waves, st)) return rc;
+    const int rc = p.waves ? attend_few(j, a->q, a->out, a->dtype, cache->format, a->max_q, p.waves, st)
+                           : attend_many(j, a->q, a->out, a->dtype, cache->format, a->max_q, st);
+    if (rc) return rc;
     return p.splits > 1 ? attend_join(j, a->out, a->dtype, a->max_q, p.block_rows, p.hd_pad, st) : VDA_OK;
 }

@@ -1,0 +1,377 @@
+// Attention over the token cache for many query rows per key head (the tokens of a frame).
+//
+// One workgroup = 4 waves = 128 query rows of one (sequence, key head), 32 for each wave; tiles of 64 keys.  The codes of the next tile
+// go from global memory to registers while this tile is multiplied, become IEEE halves times the power of two of their row, and
+// are stored in LDS once for the four waves, in a second buffer: one barrier per tile.  Scores are S^T = K Q^T (mfma 32x32x16), so a
+// query lives on a lane, the softmax needs one exchange (lane ^ 32) and only where a maximum grows, and the probabilities
+// are as they stand the B operand of O^T += V^T P^T, whose V^T operand the transposed LDS read gathers in the same key order.
+// What bounds it is vector instruction issue: about five instructions per score, one of them the exponential, against two matrix
+// instructions of 32 cycles per 1024 scores and 16 channels.
+//
+// Rows of the cache carry powers of two of any size, halves do not: the halves of a part of the key axis are relative to its
+// largest key exponent and its largest value exponent, found by a pass over the exponent bytes (a 33rd of the codes'
+// bytes) before the first tile.  A code is exact down to 2^-31 of that; below it the error is 2^-39 of the largest value.
+#include "cached_attention.h"
+
+namespace {
+
+constexpr int TK = 64;                                            // keys of a tile
+
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// byte offset of 16-byte chunk `chunk` of key `row` in the K tile [64][HDP] of halves: the sixteen rows that are read together fall
+// into the sixteen slots of a 256-byte bank row
+template <int HDP>
+__device__ __forceinline__ int ktile(int row, int chunk) {
+    const int swz = HDP == 64 ? (row >> 1) & 7 : HDP == 128 ? row & 15 : (row >> 2) & 3;
+    return row * (2 * HDP) + ((chunk ^ swz) << 4);
+}
+// byte offset of (key, byte column) in the V tile: four rows' 64-byte pieces, read transposed together, fall into different banks
+template <int HDP>
+__device__ __forceinline__ int vtile(int row, int col) {
+    const int swz = HDP == 64 ? ((row >> 1) & 1) << 6 : HDP == 128 ? (row & 3) << 6 : 0;
+    return row * (2 * HDP) + (col ^ swz);
+}
+
+// Sixteen codes times 2^e as halves; e <= 8, below -24 the factor is 0 for integers.
+template <int FMT>
+__device__ __forceinline__ void scaled16(u32x4 w, int e, f16x8& lo, f16x8& hi) {
+    f16x2 h[8];
+    if (FMT == VDA_CACHE_I8) {
+        const f16 s = (f16)__builtin_amdgcn_ldexpf(1.f, e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            codes4<FMT>(w[i], h[2 * i], h[2 * i + 1]);
+            h[2 * i] *= f16x2{s, s};
+            h[2 * i + 1] *= f16x2{s, s};
+        }
+    } else {
+        const float s = __builtin_amdgcn_ldexpf(1.f, e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            h[2 * i] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], s, false));
+            h[2 * i + 1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], s, true));
+        }
+    }
+    lo = f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+    hi = f16x8{h[4][0], h[4][1], h[5][0], h[5][1], h[6][0], h[6][1], h[7][0], h[7][1]};
+}
+
+template <typename T, int HDP, int FMT>
+__global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void attend_many_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int groups) {
+    constexpr int NP = Pieces<T>::n, KS = HDP / 16, DB = HDP / 32, CPR = HDP / 16, NC = (HDP + 63) / 64, SHIFT = FMT == VDA_CACHE_I8 ? 8 : 6;
+    constexpr int PLANE = TK * HDP * 2, BUF = 2 * PLANE;
+    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+    __shared__ uint8_t hide[2][TK];
+    __shared__ int wave_top[8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    // row blocks of one (sequence, key head, split) follow each other on one XCD and share its copy of the keys
+    int id = xcd_contiguous(blockIdx.x, groups);
+    const int rb = id % j.row_blocks;
+    id /= j.row_blocks;
+    const int split = id % j.splits;
+    id /= j.splits;
+    const int kvh = id % j.kv_heads, s = id / j.kv_heads;
+    const Span sp = span_of(j, s, max_q);
+    const int n_rho = sp.nq * j.group;
+    if (rb * 128 >= n_rho) return;                                // the whole workgroup
+    const int rho = rb * 128 + wave * 32 + r;
+    const bool live = rho < n_rho;
+    const int token = rho / j.group, head = kvh * j.group + (rho - token * j.group);
+    const long row = sp.q0 + (live ? token : 0);
+
+    // keys that a row, the wave's rows, the workgroup's rows see
+    int limit = live ? sp.n : 0, least = live ? sp.n : 0x7fffffff, most;
+    if (j.visible && live) limit = least = max(0, min(limit, j.visible[row]));
+    most = limit;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        most = max(most, __shfl_xor(most, o));
+        least = min(least, __shfl_xor(least, o));
+    }
+    if (lane == 0) wave_top[wave] = most;
+    least = __builtin_amdgcn_readfirstlane(least);
+    __syncthreads();
+    most = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
+    __syncthreads();
+    const int tiles = (most + TK - 1) / TK, per = (tiles + j.splits - 1) / j.splits;
+    const int k_begin = min(split * per, tiles) * TK, k_end = min(k_begin + per * TK, most);
+
+    const int* table = j.page_table + (long)s * j.max_pages;
+    // the row of a plane where key `key` of this sequence lies, -1 without a page
+    auto plane_row = [&](int pi, int off) -> long {
+        const int page = table[pi];
+        return page >= 0 && page < j.pages ? ((long)page * j.kv_heads + kvh) * j.page_size + off : -1L;
+    };
+
+    // the largest exponents of the part's keys and values
+    int k_ref, v_ref;
+    {
+        int tk = 1, tv = 1;
+        for (int b = (k_begin >> 4) + tid; b * 16 < k_end; b += 256) {
+            const int key = b * 16, pi = key / j.page_size;
+            const long at = plane_row(pi, key - pi * j.page_size);
+            if (at < 0) continue;
+            const u32x4 e = *reinterpret_cast<const u32x4*>(j.k_exp + at), w = *reinterpret_cast<const u32x4*>(j.v_exp + at);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int be = byte_of(e[i >> 2], i & 3), bw = byte_of(w[i >> 2], i & 3);
+                if (key + i < k_end && be != 0 && be != 255 && bw != 255) { tk = max(tk, be); tv = max(tv, bw); }
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { tk = max(tk, __shfl_xor(tk, o)); tv = max(tv, __shfl_xor(tv, o)); }
+        if (lane == 0) { wave_top[wave] = tk; wave_top[4 + wave] = tv; }
+        __syncthreads();
+        k_ref = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
+        v_ref = max(max(wave_top[4], wave_top[5]), max(wave_top[6], wave_top[7]));
+    }
+
+    f16x8 qf[KS][NP];
+    float c_row;                                                  // from products of halves to octaves
+    {
+        float f[KS][8], amax = 0.f;
+        const T* qr = q + row * j.ldq + (long)head * j.hd;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            const int e = 16 * i + 8 * h;
+            query8<T>(qr + e, live && e < j.hd, f[i]);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) amax = fmaxf(amax, fabsf(f[i][x]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int shift = query_shift(amax);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) query_pieces<NP>(f[i], shift, qf[i]);
+        c_row = __builtin_amdgcn_ldexpf(j.scale_log2e, k_ref - 127 - SHIFT - shift);
+    }
+
+    // staging: wave w brings the sixteen keys 16 w .. 16 w + 15 of every tile, which lie in one page, part i of a lane being the codes
+    // of one 16-byte chunk of one key (HDP 32: lanes 0 .. 31 bring K, the others V)
+    int s_key[NC], s_col[NC], s_k[NC], s_v[NC];                   // key of the block, byte of its row, places in the K and V tiles
+    bool s_on[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int idx = HDP == 32 ? lane & 31 : i * 64 + lane;
+        s_on[i] = idx < 16 * CPR;
+        s_key[i] = s_on[i] ? idx / CPR : 15;
+        const int c = idx % CPR;
+        s_col[i] = min(16 * c, j.row_bytes - 16);                 // padding channels meet zeros of q, or are not stored
+        s_k[i] = ktile<HDP>(16 * wave + s_key[i], 2 * c);
+        s_v[i] = PLANE + vtile<HDP>(16 * wave + s_key[i], 32 * c);
+    }
+    const bool do_k = HDP != 32 || lane < 32, do_v = HDP != 32 || lane >= 32;
+    int pi = (k_begin + 16 * wave) / j.page_size, off = k_begin + 16 * wave - pi * j.page_size;
+    const int step_pages = TK / j.page_size, step_off = TK - step_pages * j.page_size;
+    long at = -1;                                                 // the block's first row in the planes, -1 without a page
+    u32x4 k_code[NC], v_code[NC];
+    int k_exp[NC], v_exp[NC], in_block = 0;                       // in_block: keys of the block that are there
+    auto locate = [&](int k0) {                                   // the tile at k0; advances to the next one
+        in_block = min(16, k_end - k0 - 16 * wave);
+        at = in_block > 0 ? plane_row(pi, off) : -1L;
+        pi += step_pages;
+        off += step_off;
+        if (off >= j.page_size) { off -= j.page_size; ++pi; }
+    };
+    auto fetch = [&]() {
+        const long a = at < 0 ? 0 : at;                           // (rows 0 .. 15 exist; what they hold is not used)
+        const uint8_t *kr = j.k + a * j.row_bytes, *vr = j.v + a * j.row_bytes;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int o = s_key[i] * j.row_bytes + s_col[i];
+            if (HDP == 32) {
+                k_code[i] = *reinterpret_cast<const u32x4*>((do_k ? kr : vr) + o);
+                v_code[i] = k_code[i];
+            } else {
+                k_code[i] = *reinterpret_cast<const u32x4*>(kr + o);
+                v_code[i] = *reinterpret_cast<const u32x4*>(vr + o);
+            }
+            k_exp[i] = j.k_exp[a + s_key[i]];
+            v_exp[i] = j.v_exp[a + s_key[i]];
+            if (at < 0 || s_key[i] >= in_block) k_exp[i] = 0;
+        }
+    };
+    auto store = [&](int buf) {
+        char* b = smem + buf * BUF;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const bool nan = k_exp[i] == 255 || v_exp[i] == 255, gone = nan || k_exp[i] == 0;
+            // hidden: value 0 and a score that is not looked at; not a number: value 0, score NaN
+            const f16 z = nan && k_exp[i] != 0 ? (f16)__builtin_nanf("") : (f16)0.f;
+            f16x8 lo, hi;
+            if (do_k && s_on[i]) {
+                scaled16<FMT>(k_code[i], k_exp[i] - k_ref + SHIFT, lo, hi);
+                if (gone) lo = hi = f16x8{z, z, z, z, z, z, z, z};
+                *reinterpret_cast<f16x8*>(b + s_k[i]) = lo;
+                *reinterpret_cast<f16x8*>(b + (s_k[i] ^ 16)) = hi;
+            }
+            if (do_v && s_on[i]) {
+                scaled16<FMT>(v_code[i], v_exp[i] - v_ref + SHIFT, lo, hi);
+                if (gone) lo = hi = f16x8{};
+                *reinterpret_cast<f16x8*>(b + s_v[i]) = lo;       // (the V swizzle moves 64-byte pieces)
+                *reinterpret_cast<f16x8*>(b + s_v[i] + 16) = hi;
+            }
+            if (do_k && s_on[i] && s_col[i] == 0) hide[buf][16 * wave + s_key[i]] = k_exp[i] == 0;
+        }
+    };
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
+    // scores are formed relative to the running maximum (0 until the row has seen a key: then it moves there whatever its sign)
+    float m_run = 0.f, l_run = 0.f;                               // l_run: of probabilities times 2^P_SHIFT
+    bool unset = true;
+
+    if (k_begin < k_end) {
+        locate(k_begin);
+        fetch();
+        locate(k_begin + TK);
+        store(0);
+    }
+    __syncthreads();
+    const int tq = (lane & 15) >> 2, tp = lane & 3, tcol = 2 * (16 * ((lane >> 4) & 1) + 4 * tp);
+    int cur = 0;
+    for (int k0 = k_begin; k0 < k_end; k0 += TK, cur ^= 1) {
+        const bool more = k0 + TK < k_end;
+        if (more) {
+            fetch();
+            locate(k0 + 2 * TK);
+        }
+        const char* kb = smem + cur * BUF;
+        const char* vb = kb + PLANE;
+        f32x16 sc[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) sc[b][x] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const f16x8 kf = *reinterpret_cast<const f16x8*>(kb + ktile<HDP>(32 * b + r, 2 * i + h));
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) sc[b] = mfma32(kf, qf[i][p], sc[b]);
+            }
+        }
+        const unsigned long hidden = __builtin_amdgcn_ballot_w64(hide[cur][lane] != 0);
+        const unsigned hide_lo = (unsigned)hidden, hide_hi = (unsigned)(hidden >> 32);
+        const float base = (float)P_SHIFT - m_run;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) sc[b][x] = fmaf(sc[b][x], c_row, base);
+        if ((hide_lo | hide_hi) != 0 || k0 + TK > least) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const unsigned mine = (b ? hide_hi : hide_lo) >> (4 * h);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const int in32 = (x & 3) + 8 * (x >> 2);      // + 4 h
+                    if ((mine >> in32 & 1) || k0 + 32 * b + in32 + 4 * h >= limit) sc[b][x] = -INFINITY;
+                }
+            }
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sc[0][x]);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[1][x]);
+        if (__builtin_amdgcn_ballot_w64(mx > DEFER + P_SHIFT || (unset && mx > -INFINITY)) != 0) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32)) - P_SHIFT;
+            const float delta = !unset ? fmaxf(mx, 0.f) : mx == -INFINITY ? 0.f : mx, alpha = unset ? 1.f : __builtin_amdgcn_exp2f(-delta);
+            unset = unset && mx == -INFINITY;
+            m_run += delta;
+            l_run *= alpha;
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[i][x] *= alpha;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) sc[b][x] -= delta;
+        }
+        f16x8 pf[2][2][NP];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const float p = __builtin_amdgcn_exp2f(sc[b][x]);
+                sum[x & 3] += p;
+                const f16 hi = (f16)p;
+                pf[b][x >> 3][0][x & 7] = hi;
+                if (NP == 2) pf[b][x >> 3][NP - 1][x & 7] = (f16)(p - (float)hi);
+            }
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int key = 32 * b + 16 * x + 4 * h + tq;
+                    const f16x4 lo = read_tr<f16>(vb + vtile<HDP>(key, 64 * i + tcol)), hi = read_tr<f16>(vb + vtile<HDP>(key + 8, 64 * i + tcol));
+                    const f16x8 vf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) o[i] = mfma32(vf, pf[b][x][p], o[i]);
+                }
+        if (more) store(cur ^ 1);
+        __syncthreads();
+    }
+
+    // lane (r, h) holds channels 32 i + 8 g + 4 h + 0..3 of query r in o[i][4 g + 0..3]
+    const float l = l_run + __shfl_xor(l_run, 32);
+    if (!live) return;
+    if (j.splits > 1) {
+        float* p = j.part + ((((long)s * j.row_blocks + rb) * j.kv_heads + kvh) * j.splits + split) * (128 * (HDP + 2));
+        const int in_block = wave * 32 + r;
+        float* d = p + in_block * HDP + 4 * h;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 v;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[x] = __builtin_amdgcn_ldexpf(o[i][4 * g + x], v_ref - 127 - SHIFT);
+                *reinterpret_cast<f32x4*>(d + 32 * i + 8 * g) = v;
+            }
+        if (h == 0) { p[128 * HDP + in_block] = unset ? LOWEST : m_run; p[128 * HDP + 128 + in_block] = l; }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* orow = out + row * j.ldo + (long)head * j.hd + 4 * h;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (32 * i + 8 * g >= j.hd) continue;
+            typename Vec<T>::v4 v;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = (T)(__builtin_amdgcn_ldexpf(o[i][4 * g + x], v_ref - 127 - SHIFT) * inv);
+            *reinterpret_cast<typename Vec<T>::v4*>(orow + 32 * i + 8 * g) = v;
+        }
+}
+
+template <typename T>
+int many(const AttendJob& j, const T* q, T* out, int format, int max_q, hipStream_t st) {
+    const int groups = j.seqs * j.kv_heads * j.row_blocks * j.splits;
+#define VDA_M2(H, F) hipLaunchKernelGGL((attend_many_kernel<T, H, F>), dim3(groups), dim3(256), 0, st, q, out, j, max_q, groups)
+#define VDA_M(H) do { if (format == VDA_CACHE_I8) VDA_M2(H, VDA_CACHE_I8); else VDA_M2(H, VDA_CACHE_E4M3); } while (0)
+    if (j.hd <= 32) VDA_M(32);
+    else if (j.hd <= 64) VDA_M(64);
+    else if (j.hd <= 96) VDA_M(96);
+    else VDA_M(128);
+#undef VDA_M
+#undef VDA_M2
+    return hip_rc(hipGetLastError());
+}
+
+}  // namespace
+
+int attend_many(const AttendJob& j, const void* q, void* out, int dtype, int format, int max_q, hipStream_t st) {
+    if (dtype == VDA_T_BF16) return many(j, (const bf16*)q, (bf16*)out, format, max_q, st);
+    if (dtype == VDA_T_F16) return many(j, (const f16*)q, (f16*)out, format, max_q, st);
+    return many(j, (const float*)q, (float*)out, format, max_q, st);
+}

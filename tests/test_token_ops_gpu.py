@@ -290,6 +290,9 @@ def queries(rows, heads, hd, dt, seed, size=1.0):
     ([300], [40], 1, 1, 128, 1376),
     ([140], [37], 2, 2, 96, 16),
     ([64], [64], 1, 1, 8, 16),
+    ([1300, 700], [70, 100], 6, 2, 64, 64),                # several row blocks, the keys in parts
+    ([2000, 40], [6, 4], 8, 2, 32, 32),
+    ([1100], [140], 2, 2, 128, 16),
 ])
 def test_attention_over_the_cache(kv_len, q_len, heads, kv_heads, hd, page, dt, fmt):
     m = Memory(kv_len, kv_heads, hd, page, fmt, 11)

@@ -5,7 +5,7 @@
 namespace {
 
 struct Plan {
-    int row_blocks, splits, waves, block_rows, hd_pad;
+    int row_blocks, splits, chunk, waves, block_rows, hd_pad;
     long work;
 };
 
@@ -14,7 +14,7 @@ struct Plan {
 // are fewer, four waves share an item and the key axis is split over workgroups, down to 128 keys for each wave.
 // More rows: the kernel whose workgroups of 128 rows share decoded tiles; the key axis is split, down to 512 keys, until the
 // workgroups that a CU holds at once (three, two for wide heads) are there.
-constexpr int FEW_ROWS = 32;
+constexpr int FEW_ROWS = 32, MIN_FEW = 256, MIN_MANY = 512;
 int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int heads, Plan* p) {
     if (const int rc = cache_check(c)) return rc;
     if (seqs <= 0 || max_pages <= 0 || max_q <= 0 || heads <= 0) return VDA_EINVAL;
@@ -25,17 +25,26 @@ int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int head
     p->hd_pad = (c->hd + 31) & ~31;
     const long blocks = (rows + p->block_rows - 1) / p->block_rows, items = blocks * seqs * c->kv_heads;
     if (rows > 0x7fffffffL || items > 0x3fffffffL) return VDA_ESHAPE;
-    long splits;
+    // keys of a part: in few-row calls a multiple of 128 (32 for each of four waves), else of 64
+    long chunk = keys;
     if (few) {
-        const long target = 4096;
-        p->waves = items >= target || keys <= 64 ? 1 : 4;
-        splits = p->waves == 1 ? 1 : target / (items * 4);
+        p->waves = items >= 4096 || keys <= 64 ? 1 : 4;
+        if (p->waves == 4) {
+            const long wanted = 2048 / items;                     // parts, if there are keys enough
+            chunk = wanted <= 1 ? keys : (keys + wanted - 1) / wanted;
+            chunk = chunk < MIN_FEW ? MIN_FEW : chunk;
+        }
     } else {
         p->waves = 0;
-        splits = 256 * (c->hd <= 64 ? 3 : 2) / items;
+        const long wanted = 256 * (c->hd <= 64 ? 3 : 2) / items;
+        chunk = wanted <= 1 ? keys : (keys + wanted - 1) / wanted;
+        chunk = chunk < MIN_MANY ? MIN_MANY : chunk;
     }
-    splits = splits > keys / 512 ? keys / 512 : splits;
-    p->splits = (int)(splits < 1 ? 1 : splits);
+    chunk = (chunk + 127) & ~127L;
+    if (chunk > 0x40000000L) return VDA_ESHAPE;
+    const long splits = (keys + chunk - 1) / chunk;
+    p->chunk = (int)chunk;
+    p->splits = (int)splits;
     p->row_blocks = (int)blocks;
     p->work = p->splits == 1 ? 0 : items * p->splits * p->block_rows * (p->hd_pad + 2) * (long)sizeof(float);
     if (items * p->splits > 0x7fffffffL) return VDA_ESHAPE;
@@ -64,7 +73,7 @@ extern "C" int vda_cached_attention(const VdaTokenCache* cache, const VdaCachedA
     }
     const AttendJob j{(const uint8_t*)cache->k, (const uint8_t*)cache->v, cache->k_exp, cache->v_exp, a->page_table, a->kv_len, a->q_start, a->visible,
                       (float*)a->work, a->rows, a->ldq, a->ldo, cache->pages, cache->page_size, cache->kv_heads, cache->hd, cache_row_bytes(cache->hd),
-                      a->max_pages, a->heads / cache->kv_heads, a->seqs, p.row_blocks, p.splits, a->scale * 1.4426950408889634f};
+                      a->max_pages, a->heads / cache->kv_heads, a->seqs, p.row_blocks, p.splits, p.chunk, a->scale * 1.4426950408889634f};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int rc = p.waves ? attend_few(j, a->q, a->out, a->dtype, cache->format, a->max_q, p.waves, st)
                            : attend_many(j, a->q, a->out, a->dtype, cache->format, a->max_q, st);

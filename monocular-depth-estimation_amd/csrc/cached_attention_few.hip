@@ -32,7 +32,7 @@ template <int HDP> struct Step {
 
 // W waves share a (sequence, key head, row block, split) item, each with a part of its keys; W = 1: a wave per item.
 template <typename T, int HDP, int FMT, int W>
-__global__ __launch_bounds__(256) void attend_few_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int items) {
+__global__ __launch_bounds__(256, HDP == 32 ? (Pieces<T>::n == 2 ? 4 : 5) : HDP == 64 ? 4 : HDP == 96 ? 3 : 2) void attend_few_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int items) {
     constexpr int NP = Pieces<T>::n, C64 = HDP / 64, TAIL32 = (HDP / 32) & 1, CB = HDP / 32;
     constexpr int JOIN = W == 1 ? 0 : W * (HDP * 16 + 32) * 4, TILES = 4 * 32 * HDP;
     __shared__ __attribute__((aligned(16))) char smem[JOIN > TILES ? JOIN : TILES];
@@ -43,43 +43,26 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const T* __restrict__ q
     const int split = id % j.splits;
     const int item = id / j.splits;
     const int kvh = item % j.kv_heads, t0 = item / j.kv_heads, rb = t0 % j.row_blocks, s = t0 / j.row_blocks;
+    const int* table = j.page_table + (long)s * j.max_pages;
+    int first_page = W == 1 ? table[0] : -1;                        // (asked for before the lengths are known)
     const Span sp = span_of(j, s, max_q);
     const int rho = rb * 16 + c16, n_rho = sp.nq * j.group;
-    if (rb * 16 >= n_rho) return;                                   // the whole workgroup
+    if (rb * 16 >= n_rho || split * j.chunk >= max(sp.n, 1)) return;      // the whole workgroup
     const int token = rho / j.group, head = kvh * j.group + (rho - token * j.group);
     const bool live = rho < n_rho;
     const long row = sp.q0 + (live ? token : 0);
     int limit = live ? sp.n : 0;
     if (j.visible && live) limit = max(0, min(limit, j.visible[row]));
 
-    // the keys that any row of the block sees, dealt to the splits and waves in runs of whole steps
+    // the split's keys that any row of the block sees, a run of whole steps for each wave
     int most = limit;
+    if (j.visible) {
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o));
-    most = __builtin_amdgcn_readfirstlane(most);
-    const int parts = j.splits * W, steps = (most + 31) / 32, per = (steps + parts - 1) / parts;
-    const int part = split * W + (W == 1 ? 0 : wave);
-    const int k_begin = min(part * per, steps) * 32, k_end = min(k_begin + per * 32, most);
-
-    f16x8 qf[2 * C64 + TAIL32][NP];
-    float c_row;
-    {
-        float f[2 * C64 + TAIL32][8], amax = 0.f;
-        const T* qr = q + row * j.ldq + (long)head * j.hd;
-#pragma unroll
-        for (int i = 0; i < 2 * C64 + TAIL32; ++i) {
-            const int e = i < 2 * C64 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 64 * C64 + 8 * g;
-            query8<T>(qr + e, live && e < j.hd, f[i]);
-#pragma unroll
-            for (int x = 0; x < 8; ++x) amax = fmaxf(amax, fabsf(f[i][x]));
-        }
-        amax = fmaxf(amax, __shfl_xor(amax, 16));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
-        const int shift = query_shift(amax);
-#pragma unroll
-        for (int i = 0; i < 2 * C64 + TAIL32; ++i) query_pieces<NP>(f[i], shift, qf[i]);
-        c_row = __builtin_amdgcn_ldexpf(j.scale_log2e, -shift);
+        for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o));
     }
+    most = __builtin_amdgcn_readfirstlane(most);                    // (lane 0's row is there)
+    const int share = W == 1 ? j.chunk : j.chunk / W;
+    const int k_begin = split * j.chunk + (W == 1 ? 0 : wave * share), k_end = min(k_begin + share, most);
 
     // this lane's part of a V tile: it copies 16 bytes of HDP / 32 keys
     char* vt = smem + wave * (32 * HDP);
@@ -96,11 +79,10 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const T* __restrict__ q
 
     // the pages of a step's two blocks of 16 keys (a page holds a multiple of 16 slots); a block without one reads as empty slots
     int pi = k_begin / j.page_size, off = k_begin - pi * j.page_size;
-    const int* table = j.page_table + (long)s * j.max_pages;
     auto block_row = [&](int key) -> long {
         long r = -1;
         if (key < k_end) {
-            const int page = table[pi];
+            const int page = W == 1 && pi == 0 ? first_page : table[pi];
             if (page >= 0 && page < j.pages) r = ((long)page * j.kv_heads + kvh) * j.page_size + off;
         }
         off += 16;
@@ -134,7 +116,27 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const T* __restrict__ q
     int v_ref = 1;                                                  // largest exponent byte of V so far, the same in every lane
 
     Step<HDP> now, next;
-    if (k_begin < k_end) fetch(now, k_begin);
+    if (k_begin < k_end) fetch(now, k_begin);                       // in flight while q is brought into shape
+    f16x8 qf[2 * C64 + TAIL32][NP];
+    float c_row;
+    {
+        float f[2 * C64 + TAIL32][8], amax = 0.f;
+        const T* qr = q + row * j.ldq + (long)head * j.hd;
+#pragma unroll
+        for (int i = 0; i < 2 * C64 + TAIL32; ++i) {
+            const int e = i < 2 * C64 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 64 * C64 + 8 * g;
+            query8<T>(qr + e, live && e < j.hd, f[i]);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) amax = fmaxf(amax, fabsf(f[i][x]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 16));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int shift = query_shift(amax);
+#pragma unroll
+        for (int i = 0; i < 2 * C64 + TAIL32; ++i) query_pieces<NP>(f[i], shift, qf[i]);
+        c_row = __builtin_amdgcn_ldexpf(j.scale_log2e, -shift);
+    }
+
     for (int k0 = k_begin; k0 < k_end; k0 += 32) {
         if (k0 + 32 < k_end) fetch(next, k0 + 32);
         // V codes to LDS (in the order of the keys); the wave alone reads them, LDS operations of a wave stay in order
@@ -308,29 +310,35 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const T* __restrict__ q
     }
 }
 
-// The parts of a row block joined in their order: out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.  One workgroup per item.
+// The parts of a row block joined in their order: out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, the maximum m found on the way.
+// A thread per row and four channels; grid (item, run of rows).
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(T* __restrict__ out, AttendJob j, int max_q, int block_rows, int hdp) {
     const int item = blockIdx.x, kvh = item % j.kv_heads, t0 = item / j.kv_heads, rb = t0 % j.row_blocks, s = t0 / j.row_blocks;
     const Span sp = span_of(j, s, max_q);
-    const int rows = min(block_rows, sp.nq * j.group - rb * block_rows), quads = j.hd / 4;
+    const int rows = min(block_rows, sp.nq * j.group - rb * block_rows), quads = j.hd / 4, per = 256 / quads;
+    const int r0 = threadIdx.x / quads, r = blockIdx.y * per + r0, d = (threadIdx.x - r0 * quads) * 4;
+    if (r0 >= per || r >= rows) return;
     const long stride = (long)block_rows * (hdp + 2);
     const float* p = j.part + (long)item * j.splits * stride;
-    for (int i = threadIdx.x; i < rows * quads; i += 256) {
-        const int r = i / quads, d = (i - r * quads) * 4;
-        float m = LOWEST, l = 0.f;
-        for (int x = 0; x < j.splits; ++x) m = fmaxf(m, p[x * stride + block_rows * hdp + r]);
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int x = 0; x < j.splits; ++x) {
-            const float a = __builtin_amdgcn_exp2f(p[x * stride + block_rows * hdp + r] - m);
-            l += a * p[x * stride + block_rows * hdp + block_rows + r];
-            o += a * *reinterpret_cast<const f32x4*>(p + x * stride + r * hdp + d);
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int rho = rb * block_rows + r, token = rho / j.group;
-        const typename Vec<T>::v4 y = {(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
-        *reinterpret_cast<typename Vec<T>::v4*>(out + (sp.q0 + token) * j.ldo + (long)(kvh * j.group + rho - token * j.group) * j.hd + d) = y;
+    const int parts = max(1, (sp.n + j.chunk - 1) / j.chunk);
+    float m = LOWEST, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int x = 0; x < parts; ++x) {
+        const float* px = p + x * stride;
+        const float mx = px[block_rows * hdp + r], lx = px[block_rows * hdp + block_rows + r];
+        const f32x4 ox = *reinterpret_cast<const f32x4*>(px + r * hdp + d);
+        if (lx == 0.f) continue;
+        const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(mx - mn);
+        m = mn;
+        l = a * l + b * lx;
+        o = a * o + b * ox;
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int rho = rb * block_rows + r, token = rho / j.group;
+    const typename Vec<T>::v4 y = {(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+    *reinterpret_cast<typename Vec<T>::v4*>(out + (sp.q0 + token) * j.ldo + (long)(kvh * j.group + rho - token * j.group) * j.hd + d) = y;
 }
 
 template <typename T>
@@ -359,7 +367,8 @@ int attend_few(const AttendJob& j, const void* q, void* out, int dtype, int form
 }
 
 int attend_join(const AttendJob& j, void* out, int dtype, int max_q, int block_rows, int hd_pad, hipStream_t st) {
-    const dim3 grid(j.seqs * j.kv_heads * j.row_blocks);
+    const int per = 256 / (j.hd / 4);
+    const dim3 grid(j.seqs * j.kv_heads * j.row_blocks, (block_rows + per - 1) / per);
     if (dtype == VDA_T_BF16) hipLaunchKernelGGL((attend_join_kernel<bf16>), grid, dim3(256), 0, st, (bf16*)out, j, max_q, block_rows, hd_pad);
     else if (dtype == VDA_T_F16) hipLaunchKernelGGL((attend_join_kernel<f16>), grid, dim3(256), 0, st, (f16*)out, j, max_q, block_rows, hd_pad);
     else hipLaunchKernelGGL((attend_join_kernel<float>), grid, dim3(256), 0, st, (float*)out, j, max_q, block_rows, hd_pad);

@@ -57,7 +57,7 @@ __device__ __forceinline__ void scaled16(u32x4 w, int e, f16x8& lo, f16x8& hi) {
     hi = f16x8{h[4][0], h[4][1], h[5][0], h[5][1], h[6][0], h[6][1], h[7][0], h[7][1]};
 }
 
-template <typename T, int HDP, int FMT>
+template <typename T, int HDP, int FMT, int NQ>
 __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void attend_many_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int groups) {
     constexpr int NP = Pieces<T>::n, KS = HDP / 16, DB = HDP / 32, CPR = HDP / 16, NC = (HDP + 63) / 64, SHIFT = FMT == VDA_CACHE_I8 ? 8 : 6;
     constexpr int PLANE = TK * HDP * 2, BUF = 2 * PLANE;
@@ -75,16 +75,22 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
     const int kvh = id % j.kv_heads, s = id / j.kv_heads;
     const Span sp = span_of(j, s, max_q);
     const int n_rho = sp.nq * j.group;
-    if (rb * 128 >= n_rho) return;                                // the whole workgroup
-    const int rho = rb * 128 + wave * 32 + r;
-    const bool live = rho < n_rho;
-    const int token = rho / j.group, head = kvh * j.group + (rho - token * j.group);
-    const long row = sp.q0 + (live ? token : 0);
-
-    // keys that a row, the wave's rows, the workgroup's rows see
-    int limit = live ? sp.n : 0, least = live ? sp.n : 0x7fffffff, most;
-    if (j.visible && live) limit = least = max(0, min(limit, j.visible[row]));
-    most = limit;
+    constexpr int BLOCK = 128 * NQ;
+    if (rb * BLOCK >= n_rho || split * j.chunk >= max(sp.n, 1)) return;      // the whole workgroup
+    bool live[NQ];
+    int head[NQ], limit[NQ], least = 0x7fffffff, most = 0;        // keys that a row, the wave's rows, the workgroup's rows see
+    long row[NQ];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+        const int rho = rb * BLOCK + (wave * NQ + b) * 32 + r, token = rho / j.group;
+        live[b] = rho < n_rho;
+        head[b] = kvh * j.group + (rho - token * j.group);
+        row[b] = sp.q0 + (live[b] ? token : 0);
+        limit[b] = live[b] ? sp.n : 0;
+        if (j.visible && live[b]) limit[b] = max(0, min(limit[b], j.visible[row[b]]));
+        if (live[b]) least = min(least, limit[b]);
+        most = max(most, limit[b]);
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         most = max(most, __shfl_xor(most, o));
@@ -95,8 +101,7 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
     __syncthreads();
     most = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
     __syncthreads();
-    const int tiles = (most + TK - 1) / TK, per = (tiles + j.splits - 1) / j.splits;
-    const int k_begin = min(split * per, tiles) * TK, k_end = min(k_begin + per * TK, most);
+    const int k_begin = split * j.chunk, k_end = min(k_begin + j.chunk, most);
 
     const int* table = j.page_table + (long)s * j.max_pages;
     // the row of a plane where key `key` of this sequence lies, -1 without a page
@@ -128,23 +133,24 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
         v_ref = max(max(wave_top[4], wave_top[5]), max(wave_top[6], wave_top[7]));
     }
 
-    f16x8 qf[KS][NP];
-    float c_row;                                                  // from products of halves to octaves
-    {
+    f16x8 qf[NQ][KS][NP];
+    float c_row[NQ];                                              // from products of halves to octaves
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
         float f[KS][8], amax = 0.f;
-        const T* qr = q + row * j.ldq + (long)head * j.hd;
+        const T* qr = q + row[b] * j.ldq + (long)head[b] * j.hd;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             const int e = 16 * i + 8 * h;
-            query8<T>(qr + e, live && e < j.hd, f[i]);
+            query8<T>(qr + e, live[b] && e < j.hd, f[i]);
 #pragma unroll
             for (int x = 0; x < 8; ++x) amax = fmaxf(amax, fabsf(f[i][x]));
         }
         amax = fmaxf(amax, __shfl_xor(amax, 32));
         const int shift = query_shift(amax);
 #pragma unroll
-        for (int i = 0; i < KS; ++i) query_pieces<NP>(f[i], shift, qf[i]);
-        c_row = __builtin_amdgcn_ldexpf(j.scale_log2e, k_ref - 127 - SHIFT - shift);
+        for (int i = 0; i < KS; ++i) query_pieces<NP>(f[i], shift, qf[b][i]);
+        c_row[b] = __builtin_amdgcn_ldexpf(j.scale_log2e, k_ref - 127 - SHIFT - shift);
     }
 
     // staging: wave w brings the sixteen keys 16 w .. 16 w + 15 of every tile, which lie in one page, part i of a lane being the codes
@@ -194,36 +200,52 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
     };
     auto store = [&](int buf) {
         char* b = smem + buf * BUF;
+        bool odd = false;                                         // some key of the block is hidden or not a number
+#pragma unroll
+        for (int i = 0; i < NC; ++i) odd |= k_exp[i] == 0 || k_exp[i] == 255 || v_exp[i] == 255;
+        const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const bool nan = k_exp[i] == 255 || v_exp[i] == 255, gone = nan || k_exp[i] == 0;
-            // hidden: value 0 and a score that is not looked at; not a number: value 0, score NaN
-            const f16 z = nan && k_exp[i] != 0 ? (f16)__builtin_nanf("") : (f16)0.f;
-            f16x8 lo, hi;
+            f16x8 k_lo, k_hi, v_lo, v_hi;
+            scaled16<FMT>(k_code[i], k_exp[i] - k_ref + SHIFT, k_lo, k_hi);
+            scaled16<FMT>(v_code[i], v_exp[i] - v_ref + SHIFT, v_lo, v_hi);
             if (do_k && s_on[i]) {
-                scaled16<FMT>(k_code[i], k_exp[i] - k_ref + SHIFT, lo, hi);
-                if (gone) lo = hi = f16x8{z, z, z, z, z, z, z, z};
-                *reinterpret_cast<f16x8*>(b + s_k[i]) = lo;
-                *reinterpret_cast<f16x8*>(b + (s_k[i] ^ 16)) = hi;
+                *reinterpret_cast<f16x8*>(b + s_k[i]) = k_lo;
+                *reinterpret_cast<f16x8*>(b + (s_k[i] ^ 16)) = k_hi;
             }
             if (do_v && s_on[i]) {
-                scaled16<FMT>(v_code[i], v_exp[i] - v_ref + SHIFT, lo, hi);
-                if (gone) lo = hi = f16x8{};
-                *reinterpret_cast<f16x8*>(b + s_v[i]) = lo;       // (the V swizzle moves 64-byte pieces)
-                *reinterpret_cast<f16x8*>(b + s_v[i] + 16) = hi;
+                *reinterpret_cast<f16x8*>(b + s_v[i]) = v_lo;     // (the V swizzle moves 64-byte pieces)
+                *reinterpret_cast<f16x8*>(b + s_v[i] + 16) = v_hi;
+            }
+            if (any_odd && s_on[i]) {     // hidden: value 0 and a score that is not looked at; not a number: value 0, score NaN
+                const bool nan = k_exp[i] == 255 || (v_exp[i] == 255 && k_exp[i] != 0);
+                const f16 z = (f16)__builtin_nanf("");
+                if (do_k && nan) {
+                    *reinterpret_cast<f16x8*>(b + s_k[i]) = f16x8{z, z, z, z, z, z, z, z};
+                    *reinterpret_cast<f16x8*>(b + (s_k[i] ^ 16)) = f16x8{z, z, z, z, z, z, z, z};
+                }
+                if (do_v && (nan || k_exp[i] == 0)) {
+                    *reinterpret_cast<f16x8*>(b + s_v[i]) = f16x8{};
+                    *reinterpret_cast<f16x8*>(b + s_v[i] + 16) = f16x8{};
+                }
             }
             if (do_k && s_on[i] && s_col[i] == 0) hide[buf][16 * wave + s_key[i]] = k_exp[i] == 0;
         }
     };
 
-    f32x16 o[DB];
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
     // scores are formed relative to the running maximum (0 until the row has seen a key: then it moves there whatever its sign)
-    float m_run = 0.f, l_run = 0.f;                               // l_run: of probabilities times 2^P_SHIFT
-    bool unset = true;
+    f32x16 o[NQ][DB];
+    float m_run[NQ], l_run[NQ];                                   // l_run: of probabilities times 2^P_SHIFT
+    bool unset[NQ];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+        m_run[b] = l_run[b] = 0.f;
+        unset[b] = true;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[b][i][x] = 0.f;
+    }
 
     if (k_begin < k_end) {
         locate(k_begin);
@@ -235,129 +257,127 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
     const int tq = (lane & 15) >> 2, tp = lane & 3, tcol = 2 * (16 * ((lane >> 4) & 1) + 4 * tp);
     int cur = 0;
     for (int k0 = k_begin; k0 < k_end; k0 += TK, cur ^= 1) {
-        const bool more = k0 + TK < k_end;
-        if (more) {
-            fetch();
-            locate(k0 + 2 * TK);
-        }
+        fetch();                                                  // of the tile after this one, or of nothing
+        locate(k0 + 2 * TK);
         const char* kb = smem + cur * BUF;
         const char* vb = kb + PLANE;
-        f32x16 sc[2];
+        const unsigned long hidden = __builtin_amdgcn_ballot_w64(hide[cur][lane] != 0);
+        // 32 keys at a time: half the registers for scores and probabilities
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int kh = 0; kh < 2; ++kh) {
+            f32x16 sc[NQ];
 #pragma unroll
-            for (int x = 0; x < 16; ++x) sc[b][x] = 0.f;
+            for (int b = 0; b < NQ; ++b)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) sc[b][x] = 0.f;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                const f16x8 kf = *reinterpret_cast<const f16x8*>(kb + ktile<HDP>(32 * b + r, 2 * i + h));
+                const f16x8 kf = *reinterpret_cast<const f16x8*>(kb + ktile<HDP>(32 * kh + r, 2 * i + h));
 #pragma unroll
-                for (int p = NP - 1; p >= 0; --p) sc[b] = mfma32(kf, qf[i][p], sc[b]);
+                for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                    for (int b = 0; b < NQ; ++b) sc[b] = mfma32(kf, qf[b][i][p], sc[b]);
             }
-        }
-        const unsigned long hidden = __builtin_amdgcn_ballot_w64(hide[cur][lane] != 0);
-        const unsigned hide_lo = (unsigned)hidden, hide_hi = (unsigned)(hidden >> 32);
-        const float base = (float)P_SHIFT - m_run;
+            const unsigned gone = (unsigned)(kh ? hidden >> 32 : hidden);
+            f16x8 pf[NQ][2][NP];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < NQ; ++b) {
+                const float base = (float)P_SHIFT - m_run[b];
 #pragma unroll
-            for (int x = 0; x < 16; ++x) sc[b][x] = fmaf(sc[b][x], c_row, base);
-        if ((hide_lo | hide_hi) != 0 || k0 + TK > least) {
+                for (int x = 0; x < 16; ++x) sc[b][x] = fmaf(sc[b][x], c_row[b], base);
+                if (gone != 0 || k0 + 32 * kh + 32 > least) {
+                    const unsigned mine = gone >> (4 * h);
+                    const int left = limit[b] - (k0 + 32 * kh + 4 * h);
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const unsigned mine = (b ? hide_hi : hide_lo) >> (4 * h);
+                    for (int x = 0; x < 16; ++x) {
+                        const int in32 = (x & 3) + 8 * (x >> 2);  // + 4 h
+                        if ((mine >> in32 & 1) || in32 >= left) sc[b][x] = -INFINITY;
+                    }
+                }
+                float mx = sc[b][0];
+#pragma unroll
+                for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sc[b][x]);
+                if (__builtin_amdgcn_ballot_w64(mx > DEFER + P_SHIFT || (unset[b] && mx > -INFINITY)) != 0) {
+                    mx = fmaxf(mx, __shfl_xor(mx, 32)) - P_SHIFT;
+                    const float delta = !unset[b] ? fmaxf(mx, 0.f) : mx == -INFINITY ? 0.f : mx, alpha = unset[b] ? 1.f : __builtin_amdgcn_exp2f(-delta);
+                    unset[b] = unset[b] && mx == -INFINITY;
+                    m_run[b] += delta;
+                    l_run[b] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < DB; ++i)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) o[b][i][x] *= alpha;
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) sc[b][x] -= delta;
+                }
+                float sum[2] = {0.f, 0.f};
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const int in32 = (x & 3) + 8 * (x >> 2);      // + 4 h
-                    if ((mine >> in32 & 1) || k0 + 32 * b + in32 + 4 * h >= limit) sc[b][x] = -INFINITY;
+                    const float p = __builtin_amdgcn_exp2f(sc[b][x]);
+                    sum[x & 1] += p;
+                    const f16 hi = (f16)p;
+                    pf[b][x >> 3][0][x & 7] = hi;
+                    if (NP == 2) pf[b][x >> 3][NP - 1][x & 7] = (f16)(p - (float)hi);
                 }
+                l_run[b] += sum[0] + sum[1];
             }
-        }
-        float mx = sc[0][0];
-#pragma unroll
-        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sc[0][x]);
-#pragma unroll
-        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[1][x]);
-        if (__builtin_amdgcn_ballot_w64(mx > DEFER + P_SHIFT || (unset && mx > -INFINITY)) != 0) {
-            mx = fmaxf(mx, __shfl_xor(mx, 32)) - P_SHIFT;
-            const float delta = !unset ? fmaxf(mx, 0.f) : mx == -INFINITY ? 0.f : mx, alpha = unset ? 1.f : __builtin_amdgcn_exp2f(-delta);
-            unset = unset && mx == -INFINITY;
-            m_run += delta;
-            l_run *= alpha;
 #pragma unroll
             for (int i = 0; i < DB; ++i)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) o[i][x] *= alpha;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) sc[b][x] -= delta;
-        }
-        f16x8 pf[2][2][NP];
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const float p = __builtin_amdgcn_exp2f(sc[b][x]);
-                sum[x & 3] += p;
-                const f16 hi = (f16)p;
-                pf[b][x >> 3][0][x & 7] = hi;
-                if (NP == 2) pf[b][x >> 3][NP - 1][x & 7] = (f16)(p - (float)hi);
-            }
-        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-        for (int i = 0; i < DB; ++i)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const int key = 32 * b + 16 * x + 4 * h + tq;
+                    const int key = 32 * kh + 16 * x + 4 * h + tq;
                     const f16x4 lo = read_tr<f16>(vb + vtile<HDP>(key, 64 * i + tcol)), hi = read_tr<f16>(vb + vtile<HDP>(key + 8, 64 * i + tcol));
                     const f16x8 vf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
-                    for (int p = NP - 1; p >= 0; --p) o[i] = mfma32(vf, pf[b][x][p], o[i]);
+                    for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                        for (int b = 0; b < NQ; ++b) o[b][i] = mfma32(vf, pf[b][x][p], o[b][i]);
                 }
-        if (more) store(cur ^ 1);
+        }
+        store(cur ^ 1);
         __syncthreads();
     }
 
-    // lane (r, h) holds channels 32 i + 8 g + 4 h + 0..3 of query r in o[i][4 g + 0..3]
-    const float l = l_run + __shfl_xor(l_run, 32);
-    if (!live) return;
-    if (j.splits > 1) {
-        float* p = j.part + ((((long)s * j.row_blocks + rb) * j.kv_heads + kvh) * j.splits + split) * (128 * (HDP + 2));
-        const int in_block = wave * 32 + r;
-        float* d = p + in_block * HDP + 4 * h;
+    // lane (r, h) holds channels 32 i + 8 g + 4 h + 0..3 of query r in o[.][i][4 g + 0..3]
+    float* part = j.part + ((((long)s * j.row_blocks + rb) * j.kv_heads + kvh) * j.splits + split) * (BLOCK * (HDP + 2));
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+        const float l = l_run[b] + __shfl_xor(l_run[b], 32);
+        if (!live[b]) continue;
+        if (j.splits > 1) {
+            const int in_block = (wave * NQ + b) * 32 + r;
+            float* d = part + in_block * HDP + 4 * h;
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f32x4 v;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] = __builtin_amdgcn_ldexpf(o[b][i][4 * g + x], v_ref - 127 - SHIFT);
+                    *reinterpret_cast<f32x4*>(d + 32 * i + 8 * g) = v;
+                }
+            if (h == 0) { part[BLOCK * HDP + in_block] = unset[b] ? LOWEST : m_run[b]; part[BLOCK * HDP + BLOCK + in_block] = l; }
+            continue;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T* orow = out + row[b] * j.ldo + (long)head[b] * j.hd + 4 * h;
 #pragma unroll
         for (int i = 0; i < DB; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                f32x4 v;
+                if (32 * i + 8 * g >= j.hd) continue;
+                typename Vec<T>::v4 v;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) v[x] = __builtin_amdgcn_ldexpf(o[i][4 * g + x], v_ref - 127 - SHIFT);
-                *reinterpret_cast<f32x4*>(d + 32 * i + 8 * g) = v;
+                for (int x = 0; x < 4; ++x) v[x] = (T)(__builtin_amdgcn_ldexpf(o[b][i][4 * g + x], v_ref - 127 - SHIFT) * inv);
+                *reinterpret_cast<typename Vec<T>::v4*>(orow + 32 * i + 8 * g) = v;
             }
-        if (h == 0) { p[128 * HDP + in_block] = unset ? LOWEST : m_run; p[128 * HDP + 128 + in_block] = l; }
-        return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* orow = out + row * j.ldo + (long)head * j.hd + 4 * h;
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            if (32 * i + 8 * g >= j.hd) continue;
-            typename Vec<T>::v4 v;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) v[x] = (T)(__builtin_amdgcn_ldexpf(o[i][4 * g + x], v_ref - 127 - SHIFT) * inv);
-            *reinterpret_cast<typename Vec<T>::v4*>(orow + 32 * i + 8 * g) = v;
-        }
 }
 
 template <typename T>
 int many(const AttendJob& j, const T* q, T* out, int format, int max_q, hipStream_t st) {
     const int groups = j.seqs * j.kv_heads * j.row_blocks * j.splits;
-#define VDA_M2(H, F) hipLaunchKernelGGL((attend_many_kernel<T, H, F>), dim3(groups), dim3(256), 0, st, q, out, j, max_q, groups)
+#define VDA_M2(H, F) hipLaunchKernelGGL((attend_many_kernel<T, H, F, 1>), dim3(groups), dim3(256), 0, st, q, out, j, max_q, groups)
 #define VDA_M(H) do { if (format == VDA_CACHE_I8) VDA_M2(H, VDA_CACHE_I8); else VDA_M2(H, VDA_CACHE_E4M3); } while (0)
     if (j.hd <= 32) VDA_M(32);
     else if (j.hd <= 64) VDA_M(64);

@@ -5,6 +5,7 @@ the C ABI and raises on a non-zero return code.  There is no fallback: if the li
 """
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -128,12 +129,13 @@ def lib():
         l.vda_colormap_bytes_u8.argtypes = [C.c_void_p] * 4 + [C.c_long, C.c_void_p]
         l.vda_warp_blend_f32.argtypes = [C.c_void_p] * 4 + [C.c_int, C.c_int, C.c_float, C.c_float, C.c_void_p]
         l.vda_rotary_axes.argtypes = [C.c_void_p] * 4 + [C.c_long, C.c_int, C.c_int, C.c_long, C.c_long] + [C.c_int] * 6 + [C.c_void_p]
-        l.vda_cache_write.argtypes = ([C.POINTER(CacheDesc)] + [C.c_void_p] * 3 + [C.c_long] * 3 + [C.c_int, C.c_void_p, C.c_void_p]
+        # (a struct by reference, or the bytes of one: see _packer)
+        l.vda_cache_write.argtypes = ([C.c_void_p] + [C.c_void_p] * 3 + [C.c_long] * 3 + [C.c_int, C.c_void_p, C.c_void_p]
                                       + [C.c_int] * 5 + [C.c_void_p])
-        l.vda_cache_read.argtypes = [C.POINTER(CacheDesc)] + [C.c_void_p] * 3 + [C.c_long] * 3 + [C.c_int, C.c_void_p]
-        l.vda_cached_attention_work.argtypes = [C.POINTER(CacheDesc)] + [C.c_int] * 4
-        l.vda_cached_attention.argtypes = [C.POINTER(CacheDesc), C.POINTER(CachedAttentionArgs), C.c_void_p]
-        l.vda_gated_norm.argtypes = [C.POINTER(GatedNormArgs), C.c_void_p]
+        l.vda_cache_read.argtypes = [C.c_void_p] + [C.c_void_p] * 3 + [C.c_long] * 3 + [C.c_int, C.c_void_p]
+        l.vda_cached_attention_work.argtypes = [C.c_void_p] + [C.c_int] * 4
+        l.vda_cached_attention.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        l.vda_gated_norm.argtypes = [C.c_void_p, C.c_void_p]
         for name in EXPORTS[1:]:
             getattr(l, name).restype = C.c_int
         l.vda_cached_attention_work.restype = C.c_long
@@ -582,40 +584,72 @@ def warp_blend_f32(prev, cur, flow, out, h, w, w_cur, w_prev):
 
 
 # ---- operators of a video transformer that works frame by frame: rotary positions, token cache, attention over it, norms -----------
+# Their smallest calls take a few microseconds on the device, so the checks here are kept to a handful of attribute reads per tensor.
 PAIR_HALVES, PAIR_ADJACENT = 0, 1                   # VDA_PAIR_*
 CACHE_E4M3, CACHE_I8 = 0, 1                         # VDA_CACHE_*
 NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2           # VDA_NORM_*
+_F32, _F64, _I32, _I64, _U8 = torch.float32, torch.float64, torch.int32, torch.int64, torch.uint8
+
+
+def _packer(struct_type):
+    """Field values -> the bytes of an argument struct, which ctypes passes by reference (a third of the time of filling the
+    ctypes structure)."""
+    code = {C.c_void_p: "P", C.c_long: "l", C.c_int: "i", C.c_float: "f"}
+    return struct.Struct("@" + "".join(code[f] for _, f in struct_type._fields_) + "0P").pack
+
+
+_pack_cache, _pack_attention, _pack_norm = _packer(CacheDesc), _packer(CachedAttentionArgs), _packer(GatedNormArgs)
 
 
 def _here(what, *ts):
     """These operators launch on the current device's current stream: all tensors have to live there."""
-    _dev(*ts)
-    here = torch.cuda.current_device() if _current_device is None else _current_device()
+    here = None
     for t in ts:
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"{what}: a tensor is on device {t.get_device()}, the current device is {here}")
+        if t is not None:
+            at = t.get_device()
+            if at != here:
+                _dev(t)
+                here = torch.cuda.current_device() if _current_device is None else _current_device()
+                if at != here:
+                    raise ValueError(f"{what}: a tensor is on device {at}, the current device is {here}")
 
 
-def _row_stride(what, name, t, width, ld):
-    """Elements from one row of ``t`` to the next: ``ld``, or what the tensor's own stride says.  Within a row values are dense."""
-    if t.dim() < 2:
-        return width if ld is None else ld
-    dense = 1
-    for n, s in zip(t.shape[:0:-1], t.stride()[:0:-1]):
-        if n != 1 and s != dense:
-            raise ValueError(f"{what}: the rows of {name} are not dense (strides {tuple(t.stride())})")
-        dense *= n
-    return (max(t.stride(0), width) if t.shape[0] > 1 else width) if ld is None else ld
+def _rows(what, name, t, rows, width, ld):
+    """(address, elements from one row to the next) of ``rows`` rows of ``width`` dense values: the stride is ``ld``, or what the
+    tensor's own says, and the tensor's memory holds them."""
+    if ld is None and t.is_contiguous() and t.numel() == rows * width:
+        return t.data_ptr(), width
+    if t.dim() >= 2:
+        dense = 1
+        for n, s in zip(t.shape[:0:-1], t.stride()[:0:-1]):
+            if n != 1 and s != dense:
+                raise ValueError(f"{what}: the rows of {name} are not dense (strides {tuple(t.stride())})")
+            dense *= n
+        if ld is None:
+            ld = max(t.stride(0), width) if t.shape[0] > 1 else width
+    elif ld is None:
+        ld = width
+    _need(what, **{name: (t, (rows - 1) * ld + width)})
+    return t.data_ptr(), ld
+
+
+def _vector(what, name, t, elements, dtype):
+    """Address of ``elements`` dense values (0 for None)."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype:
+        raise TypeError(f"{what}: {name} has to be {dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: {name} is dense")
+    if t.numel() < elements:
+        _need(what, **{name: (t, elements)})
+    return t.data_ptr()
 
 
 def _axes(what, pos, freq, sections, rows):
     n_t, n_h, n_w = sections
-    if pos.dtype not in (torch.int32, torch.float32) or freq.dtype != torch.float64:
-        raise TypeError(f"{what}: int32 or fp32 positions, float64 frequencies")
-    if not (pos.is_contiguous() and freq.is_contiguous()):
-        raise ValueError(f"{what}: pos and freq are dense")
-    _need(what, pos=(pos, 3 * rows), freq=(freq, n_t + n_h + n_w))
-    return n_t, n_h, n_w
+    p = _vector(what, "pos", pos, 3 * rows, _F32 if pos.dtype is _F32 else _I32)         # either
+    return p, _vector(what, "freq", freq, n_t + n_h + n_w, _F64), n_t, n_h, n_w
 
 
 def rotary_axes(x, out, pos, freq, *, rows, heads, hd, sections, pairing=PAIR_HALVES, ldx=None, ldo=None):
@@ -624,13 +658,13 @@ def rotary_axes(x, out, pos, freq, *, rows, heads, hd, sections, pairing=PAIR_HA
     width).  ``out`` may be ``x``.  Row strides are the tensors' own unless given.  A negated ``freq`` undoes the rotation."""
     what = "vda_rotary_axes"
     _here(what, x, out, pos, freq)
-    if x.dtype != out.dtype or x.dtype not in _TYPES:
+    dtype = _TYPES.get(x.dtype)
+    if dtype is None or out.dtype is not x.dtype:
         raise TypeError(f"{what}: x and out share one type of fp32, bf16, fp16")
-    n_t, n_h, n_w = _axes(what, pos, freq, sections, rows)
-    ldx, ldo = _row_stride(what, "x", x, heads * hd, ldx), _row_stride(what, "out", out, heads * hd, ldo)
-    _need(what, x=(x, (rows - 1) * ldx + heads * hd), out=(out, (rows - 1) * ldo + heads * hd))
-    _check(lib().vda_rotary_axes(_ptr(x), _ptr(out), _ptr(pos), _ptr(freq), rows, heads, hd, ldx, ldo, n_t, n_h, n_w, int(pairing),
-                                 int(pos.dtype == torch.float32), _type(x), _stream()), what)
+    p, f, n_t, n_h, n_w = _axes(what, pos, freq, sections, rows)
+    px, ldx = _rows(what, "x", x, rows, heads * hd, ldx)
+    po, ldo = _rows(what, "out", out, rows, heads * hd, ldo)
+    _check(lib().vda_rotary_axes(px, po, p, f, rows, heads, hd, ldx, ldo, n_t, n_h, n_w, pairing, pos.dtype is _F32, dtype, _stream()), what)
 
 
 def cache_row_bytes(hd):
@@ -639,13 +673,26 @@ def cache_row_bytes(hd):
 
 
 def _cache(what, ck, cv, ek, ev, kv_heads, hd, page_size, fmt):
-    shape = (ck.shape[0], kv_heads, page_size, cache_row_bytes(hd))
-    for t, want in ((ck, shape), (cv, shape), (ek, shape[:3]), (ev, shape[:3])):
-        if t.dtype != torch.uint8:
+    """The bytes of a VdaTokenCache over these planes."""
+    pages = ck.shape[0]
+    slots = pages * kv_heads * page_size
+    codes = slots * cache_row_bytes(hd)
+    for t, n in ((ck, codes), (cv, codes), (ek, slots), (ev, slots)):
+        if t.dtype is not _U8:
             raise TypeError(f"{what}: cache planes are uint8")
-        if tuple(t.shape) != want or not t.is_contiguous():
-            raise ValueError(f"{what}: a cache plane of shape {tuple(t.shape)}, wanted dense {want}")
-    return CacheDesc(ck.data_ptr(), cv.data_ptr(), ek.data_ptr(), ev.data_ptr(), shape[0], page_size, kv_heads, hd, int(fmt))
+        if t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{what}: a cache plane of shape {tuple(t.shape)}, wanted dense {(pages, kv_heads, page_size)} rows of "
+                             f"{n // max(slots, 1)} bytes")
+    return _pack_cache(ck.data_ptr(), cv.data_ptr(), ek.data_ptr(), ev.data_ptr(), pages, page_size, kv_heads, hd, fmt)
+
+
+def _cache_rows(what, k, v, slots, rows, width, ldk, ldv):
+    dtype = _TYPES.get(k.dtype)
+    if dtype is None or v.dtype is not k.dtype:
+        raise TypeError(f"{what}: k and v share one type of fp32, bf16, fp16")
+    pk, ldk = _rows(what, "k", k, rows, width, ldk)
+    pv, ldv = _rows(what, "v", v, rows, width, ldv)
+    return pk, pv, _vector(what, "slots", slots, rows, _I64), ldk, ldv, dtype
 
 
 def cache_write(k, v, ck, cv, ek, ev, slots, *, rows, kv_heads, hd, page_size, fmt, pos=None, freq=None, sections=None,
@@ -655,19 +702,13 @@ def cache_write(k, v, ck, cv, ek, ev, slots, *, rows, kv_heads, hd, page_size, f
     by ``rotary_axes``."""
     what = "vda_cache_write"
     _here(what, k, v, ck, cv, ek, ev, slots, pos, freq)
-    if k.dtype != v.dtype or k.dtype not in _TYPES or slots.dtype != torch.int64:
-        raise TypeError(f"{what}: k and v share one type of fp32, bf16, fp16; slots are int64")
     if (pos is None) != (freq is None) or (pos is None) != (sections is None):
         raise ValueError(f"{what}: pos, freq and sections come together")
     desc = _cache(what, ck, cv, ek, ev, kv_heads, hd, page_size, fmt)
-    n = _axes(what, pos, freq, sections, rows) if pos is not None else (0, 0, 0)
-    width = kv_heads * hd
-    ldk, ldv = _row_stride(what, "k", k, width, ldk), _row_stride(what, "v", v, width, ldv)
-    if not slots.is_contiguous():
-        raise ValueError(f"{what}: slots are dense")
-    _need(what, k=(k, (rows - 1) * ldk + width), v=(v, (rows - 1) * ldv + width), slots=(slots, rows))
-    _check(lib().vda_cache_write(C.byref(desc), _ptr(k), _ptr(v), _ptr(slots), rows, ldk, ldv, _type(k), _ptr(pos), _ptr(freq), *n, int(pairing),
-                                 int(pos is not None and pos.dtype == torch.float32), _stream()), what)
+    pk, pv, ps, ldk, ldv, dtype = _cache_rows(what, k, v, slots, rows, kv_heads * hd, ldk, ldv)
+    p, f, n_t, n_h, n_w = (None, None, 0, 0, 0) if pos is None else _axes(what, pos, freq, sections, rows)
+    _check(lib().vda_cache_write(desc, pk, pv, ps, rows, ldk, ldv, dtype, p, f, n_t, n_h, n_w, pairing, pos is not None and pos.dtype is _F32,
+                                 _stream()), what)
 
 
 def cache_read(ck, cv, ek, ev, slots, k, v, *, rows, kv_heads, hd, page_size, fmt, ldk=None, ldv=None):
@@ -675,21 +716,15 @@ def cache_read(ck, cv, ek, ev, slots, k, v, *, rows, kv_heads, hd, page_size, fm
     read as 0."""
     what = "vda_cache_read"
     _here(what, k, v, ck, cv, ek, ev, slots)
-    if k.dtype != v.dtype or k.dtype not in _TYPES or slots.dtype != torch.int64:
-        raise TypeError(f"{what}: k and v share one type of fp32, bf16, fp16; slots are int64")
     desc = _cache(what, ck, cv, ek, ev, kv_heads, hd, page_size, fmt)
-    width = kv_heads * hd
-    ldk, ldv = _row_stride(what, "k", k, width, ldk), _row_stride(what, "v", v, width, ldv)
-    if not slots.is_contiguous():
-        raise ValueError(f"{what}: slots are dense")
-    _need(what, k=(k, (rows - 1) * ldk + width), v=(v, (rows - 1) * ldv + width), slots=(slots, rows))
-    _check(lib().vda_cache_read(C.byref(desc), _ptr(slots), _ptr(k), _ptr(v), rows, ldk, ldv, _type(k), _stream()), what)
+    pk, pv, ps, ldk, ldv, dtype = _cache_rows(what, k, v, slots, rows, kv_heads * hd, ldk, ldv)
+    _check(lib().vda_cache_read(desc, ps, pk, pv, rows, ldk, ldv, dtype, _stream()), what)
 
 
 def cached_attention_work(ck, *, seqs, max_pages, max_q, heads, kv_heads, hd, page_size, fmt):
     """Bytes of scratch that ``cached_attention`` needs for these sizes."""
-    desc = CacheDesc(ck.data_ptr(), ck.data_ptr(), ck.data_ptr(), ck.data_ptr(), ck.shape[0], page_size, kv_heads, hd, int(fmt))
-    n = lib().vda_cached_attention_work(C.byref(desc), seqs, max_pages, max_q, heads)
+    p = ck.data_ptr()
+    n = lib().vda_cached_attention_work(_pack_cache(p, p, p, p, ck.shape[0], page_size, kv_heads, hd, fmt), seqs, max_pages, max_q, heads)
     _check(min(n, 0), "vda_cached_attention_work")
     return n
 
@@ -702,30 +737,33 @@ def cached_attention(q, out, ck, cv, ek, ev, page_table, kv_len, q_start, *, hea
     None takes it from torch's allocator for this call.  Rows of no sequence stay as they were; a row that sees no key is 0."""
     what = "vda_cached_attention"
     _here(what, q, out, ck, cv, ek, ev, page_table, kv_len, q_start, visible, work)
-    if q.dtype != out.dtype or q.dtype not in _TYPES:
+    dtype = _TYPES.get(q.dtype)
+    if dtype is None or out.dtype is not q.dtype:
         raise TypeError(f"{what}: q and out share one type of fp32, bf16, fp16")
-    for t in (page_table, kv_len, q_start, visible):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
-            raise TypeError(f"{what}: page_table, kv_len, q_start and visible are dense int32")
-    if page_table.dim() != 2 or page_table.shape[0] != kv_len.numel() or q_start.numel() != kv_len.numel() + 1:
+    seqs = kv_len.numel()
+    if page_table.dim() != 2 or page_table.shape[0] != seqs or q_start.numel() != seqs + 1:
         raise ValueError(f"{what}: page_table [seqs, max_pages], kv_len [seqs] and q_start [seqs + 1] belong together")
     desc = _cache(what, ck, cv, ek, ev, kv_heads, hd, page_size, fmt)
-    seqs, max_pages = page_table.shape
-    width = heads * hd
-    ldq, ldo = _row_stride(what, "q", q, width, ldq), _row_stride(what, "out", out, width, ldo)
+    max_pages = page_table.shape[1]
     rows = q.shape[0] if rows is None else rows
-    _need(what, q=(q, (rows - 1) * ldq + width), out=(out, (rows - 1) * ldo + width), visible=(visible, rows))
-    n = lib().vda_cached_attention_work(C.byref(desc), seqs, max_pages, max_q, heads)
+    pq, ldq = _rows(what, "q", q, rows, heads * hd, ldq)
+    po, ldo = _rows(what, "out", out, rows, heads * hd, ldo)
+    pt, pl = _vector(what, "page_table", page_table, 0, _I32), _vector(what, "kv_len", kv_len, 0, _I32)
+    ps, pv = _vector(what, "q_start", q_start, 0, _I32), _vector(what, "visible", visible, rows, _I32)
+    l = lib()
+    n = l.vda_cached_attention_work(desc, seqs, max_pages, max_q, heads)
     _check(min(n, 0), what)
-    if work is None:
-        work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    have = 0 if work is None else work.untyped_storage().nbytes() - work.storage_offset() * work.element_size()
-    if have < n:
-        raise ValueError(f"{what}: work holds {have} bytes, the call needs {n}")
-    a = CachedAttentionArgs(q.data_ptr(), out.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(), q_start.data_ptr(),
-                            None if visible is None else visible.data_ptr(), None if work is None else work.data_ptr(), have, rows, ldq, ldo,
-                            seqs, max_pages, max_q, heads, _type(q), float(scale))
-    _check(lib().vda_cached_attention(C.byref(desc), C.byref(a), _stream()), what)
+    have = pw = 0
+    if n:
+        if work is None:
+            work, have = torch.empty(n, dtype=_U8, device=q.device), n
+        else:
+            have = work.untyped_storage().nbytes() - work.storage_offset() * work.element_size()
+            if have < n:
+                raise ValueError(f"{what}: work holds {have} bytes, the call needs {n}")
+        pw = work.data_ptr()
+    args = _pack_attention(pq, po, pt, pl, ps, pv, pw, have, rows, ldq, ldo, seqs, max_pages, max_q, heads, dtype, scale)
+    _check(l.vda_cached_attention(desc, args, _stream()), what)
 
 
 def gated_norm(x, b, x_out, y, *, rows, C, post=NORM_NONE, post_w=None, post_b=None, gate=None, resid_scale=1.0, pre=NORM_LAYER, pre_w=None,
@@ -734,31 +772,27 @@ def gated_norm(x, b, x_out, y, *, rows, C, post=NORM_NONE, post_w=None, post_b=N
     pre_b) * (1 + mod_scale[g]) + mod_shift[g]``, g = row // rows_per_group (default: one group).  ``x``, ``x_out`` fp32 (may be the
     same), ``b`` and ``y`` of any storage type; ``b = x_out = None``: y of x alone; ``y = None`` (with pre = NORM_NONE): the update alone."""
     what = "vda_gated_norm"
-    vectors = dict(post_w=post_w, post_b=post_b, pre_w=pre_w, pre_b=pre_b)
-    grouped = dict(gate=gate, mod_scale=mod_scale, mod_shift=mod_shift)
-    _here(what, x, b, x_out, y, *vectors.values(), *grouped.values())
+    _here(what, x, b, x_out, y, post_w, post_b, gate, pre_w, pre_b, mod_scale, mod_shift)
     per = rows if rows_per_group is None else rows_per_group
     if per <= 0:
         raise ValueError(f"{what}: rows_per_group is positive")
-    groups = -(-rows // per)
-    for name, t in (("x", x), ("x_out", x_out), *vectors.items(), *grouped.items()):
-        if t is not None and t.dtype != torch.float32:
-            raise TypeError(f"{what}: {name} is fp32")
-    for name, t in (*vectors.items(), *grouped.items()):
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f"{what}: {name} is dense")
-    for t in (b, y):
-        if t is not None and t.dtype not in _TYPES:
-            raise TypeError(f"{what}: b and y are fp32, bf16 or fp16")
-    stride = lambda name, t, ld: C if t is None else _row_stride(what, name, t, C, ld)  # noqa: E731
-    ldx, ldb, ldxo, ldy = stride("x", x, ldx), stride("b", b, ldb), stride("x_out", x_out, ldxo), stride("y", y, ldy)
-    _need(what, x=(x, (rows - 1) * ldx + C), b=(b, (rows - 1) * ldb + C), x_out=(x_out, (rows - 1) * ldxo + C), y=(y, (rows - 1) * ldy + C),
-          **{n: (t, C) for n, t in vectors.items()}, **{n: (t, groups * C) for n, t in grouped.items()})
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    a = GatedNormArgs(p(x), p(b), p(x_out), p(y), p(post_w), p(post_b), p(gate), p(pre_w), p(pre_b), p(mod_scale), p(mod_shift),
-                      rows, ldx, ldb, ldxo, ldy, C, per, int(post), int(pre), T_NONE if b is None else _type(b), T_NONE if y is None else _type(y),
-                      float(resid_scale), float(eps))
-    _check(lib().vda_gated_norm(_byref(a), _stream()), what)
-
-
-_byref = C.byref          # (``C`` is the channel count inside gated_norm)
+    grouped = -(-rows // per) * C
+    if x.dtype is not _F32 or (x_out is not None and x_out.dtype is not _F32):
+        raise TypeError(f"{what}: x and x_out are fp32")
+    px, ldx = _rows(what, "x", x, rows, C, ldx)
+    pb = po = py = b_type = y_type = 0
+    if b is not None:
+        b_type = _TYPES.get(b.dtype)
+        pb, ldb = _rows(what, "b", b, rows, C, ldb)
+    if x_out is not None:
+        po, ldxo = _rows(what, "x_out", x_out, rows, C, ldxo)
+    if y is not None:
+        y_type = _TYPES.get(y.dtype)
+        py, ldy = _rows(what, "y", y, rows, C, ldy)
+    if b_type is None or y_type is None:
+        raise TypeError(f"{what}: b and y are fp32, bf16 or fp16")
+    args = _pack_norm(px, pb, po, py, _vector(what, "post_w", post_w, C, _F32), _vector(what, "post_b", post_b, C, _F32),
+                      _vector(what, "gate", gate, grouped, _F32), _vector(what, "pre_w", pre_w, C, _F32), _vector(what, "pre_b", pre_b, C, _F32),
+                      _vector(what, "mod_scale", mod_scale, grouped, _F32), _vector(what, "mod_shift", mod_shift, grouped, _F32),
+                      rows, ldx, ldb or C, ldxo or C, ldy or C, C, per, post, pre, b_type, y_type, resid_scale, eps)
+    _check(lib().vda_gated_norm(args, _stream()), what)

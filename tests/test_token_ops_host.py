@@ -95,7 +95,7 @@ def test_attention_wrapper_refusals(recorded):
     hip.cached_attention(q, q.clone(), *p, table, kv_len, start, visible=seen, **kw)
     assert recorded == ["vda_cached_attention_work", "vda_cached_attention"]
     for bad, error, match in ((dict(out=q.float()), TypeError, "share"), (dict(table=table.long()), TypeError, "int32"), (dict(seen=seen[:5].clone()), ValueError, "visible holds"),
-                              (dict(table=torch.zeros(3, 2, dtype=i32).t()), TypeError, "dense"), (dict(start=start[:2]), ValueError, "belong"),
+                              (dict(table=torch.zeros(3, 2, dtype=i32).t()), ValueError, "dense"), (dict(start=start[:2]), ValueError, "belong"),
                               (dict(kv_len=torch.zeros(3, dtype=i32)), ValueError, "belong"), (dict(out=q[:5].clone()), ValueError, "out holds"),
                               (dict(q=torch.zeros(6, 4, 48, dtype=f16)[..., ::2]), ValueError, "not dense")):
         a = {**dict(q=q, out=q.clone(), table=table, kv_len=kv_len, start=start, seen=seen), **bad}
@@ -124,7 +124,7 @@ def test_norm_wrapper_refusals(recorded):
     kw = dict(rows=6, C=32, rows_per_group=2)
     hip.gated_norm(x, b, x, b.clone(), gate=gate, pre_w=w, **kw)
     assert recorded == ["vda_gated_norm"]
-    for bad, error, match in ((dict(x=x.half()), TypeError, "x is fp32"), (dict(gate=gate[:2].clone()), ValueError, "gate holds"), (dict(gate=gate.half()), TypeError, "gate is fp32"),
+    for bad, error, match in ((dict(x=x.half()), TypeError, "fp32"), (dict(gate=gate[:2].clone()), ValueError, "gate holds"), (dict(gate=gate.half()), TypeError, "gate has to be torch.float32"),
                               (dict(gate=torch.zeros(3, 64)[:, ::2]), ValueError, "dense"), (dict(pre_w=w[:31].clone()), ValueError, "pre_w holds"),
                               (dict(b=b.to(i32)), TypeError, "b and y"), (dict(y=b[:5].clone()), ValueError, "y holds"), (dict(rows_per_group=0), ValueError, "positive"),
                               (dict(x_out=x[:5].clone()), ValueError, "x_out holds")):

@@ -2,6 +2,20 @@
 #pragma once
 #include "token_cache.h"
 
+// n / d for 0 <= n < 2^31 and a divisor known when the call is made: one high product and a shift.  With l = ceil(log2 d) and
+// m = ceil(2^(31 + l) / d) the product n m / 2^(31 + l) exceeds n / d by less than n / 2^31 < 1 of 1 / d, which reaches no next integer.
+struct Quick {
+    unsigned d, m;
+    int s;
+    explicit Quick(unsigned n) : d(n) {
+        int l = 0;
+        while ((1ull << l) < n) ++l;
+        m = (unsigned)(((1ull << (31 + l)) + n - 1) / n);
+        s = l - 1;
+    }
+    __device__ __forceinline__ int over(int n) const { return d == 1 ? n : (int)(__umulhi((unsigned)n, m) >> s); }
+};
+
 // One launch.  Query row `rho` of a sequence and key head is query token rho / group, head kvh * group + rho % group: the heads that
 // share a key head share its tiles.
 struct AttendJob {
@@ -14,6 +28,7 @@ struct AttendJob {
     int row_blocks, splits;     // blocks of query rows per (sequence, key head); parts of the key axis,
     int chunk;                  // of `chunk` keys each: a short sequence has fewer parts, not smaller ones
     float scale_log2e;
+    Quick by_splits, by_heads, by_blocks, by_group, by_page;
 };
 
 // The sequence's own numbers, cut to what the tensors hold.
@@ -90,10 +105,13 @@ __device__ __forceinline__ void query_pieces(const float* f, int shift, f16x8* o
 template <typename T> struct Pieces { static constexpr int n = 1; };
 template <> struct Pieces<float> { static constexpr int n = 2; };
 
-__device__ __forceinline__ int byte_of(unsigned w, int i) { return (w >> (8 * i)) & 255; }
-// 0x80 in every byte of w that is 0
-__device__ __forceinline__ unsigned zero_bytes(unsigned w) { return (w - 0x01010101u) & ~w & 0x80808080u; }
-__device__ __forceinline__ float power_of_byte(int byte) { return __uint_as_float((unsigned)byte << 23); }      // 2^(byte - 127), 1 <= byte <= 254
+__device__ __forceinline__ unsigned byte_of(unsigned w, int i) { return (w >> (8 * i)) & 255u; }
+// not 0 if some byte of w is 0 or 255 (and now and then for 254 above a 255: a carry; the caller then looks at each byte)
+__device__ __forceinline__ unsigned odd_bytes(unsigned w) {
+    const unsigned x = (w + 0x01010101u) & 0xfefefefeu;
+    return (x - 0x01010101u) & ~x & 0x80808080u;
+}
+__device__ __forceinline__ float power_of_byte(unsigned byte) { return __uint_as_float(byte << 23); }      // 2^(byte - 127), 1 <= byte <= 254
 
 int attend_few(const AttendJob& j, const void* q, void* out, int dtype, int format, int max_q, int waves, hipStream_t st);
 int attend_many(const AttendJob& j, const void* q, void* out, int dtype, int format, int max_q, hipStream_t st);

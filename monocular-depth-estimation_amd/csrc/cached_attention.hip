@@ -73,7 +73,8 @@ extern "C" int vda_cached_attention(const VdaTokenCache* cache, const VdaCachedA
     }
     const AttendJob j{(const uint8_t*)cache->k, (const uint8_t*)cache->v, cache->k_exp, cache->v_exp, a->page_table, a->kv_len, a->q_start, a->visible,
                       (float*)a->work, a->rows, a->ldq, a->ldo, cache->pages, cache->page_size, cache->kv_heads, cache->hd, cache_row_bytes(cache->hd),
-                      a->max_pages, a->heads / cache->kv_heads, a->seqs, p.row_blocks, p.splits, p.chunk, a->scale * 1.4426950408889634f};
+                      a->max_pages, a->heads / cache->kv_heads, a->seqs, p.row_blocks, p.splits, p.chunk, a->scale * 1.4426950408889634f,
+                      Quick(p.splits), Quick(cache->kv_heads), Quick(p.row_blocks), Quick(a->heads / cache->kv_heads), Quick(cache->page_size)};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int rc = p.waves ? attend_few(j, a->q, a->out, a->dtype, cache->format, a->max_q, p.waves, st)
                            : attend_many(j, a->q, a->out, a->dtype, cache->format, a->max_q, st);

@@ -23,6 +23,8 @@ __device__ __forceinline__ int vtile(int key, int col) {
     return key * HDP + (col ^ swz);
 }
 
+constexpr int V_REF_MIN = 40;        // smallest reference of the value exponents: values of 1e-33 and less lose bits against it
+
 template <int HDP> struct Step {
     u32x4 k[2][HDP >= 64 ? HDP / 64 : 1];         // 64 channels of a key: 16 bytes per lane
     u32x2 k8[2];                                  // 32 channels of a key: 8 bytes per lane (HDP 32 and 96)
@@ -30,39 +32,27 @@ template <int HDP> struct Step {
     unsigned ek[2], ev[2];
 };
 
+// Waves per SIMD that the registers allow without spilling (32, 64, 96, 128 channels; more pieces of q or the longer code of W = 1
+// cost one).
+template <typename T, int HDP, int FMT, int W> constexpr int few_waves() {
+    constexpr bool big = Pieces<T>::n == 2 || (W == 1 && (HDP > 32 || FMT == VDA_CACHE_E4M3));
+    return HDP == 32 ? (big ? 4 : 5) : HDP == 64 ? (big ? 3 : 4) : HDP == 96 ? (big ? 2 : 3) : 2;
+}
+
 // W waves share a (sequence, key head, row block, split) item, each with a part of its keys; W = 1: a wave per item.
 template <typename T, int HDP, int FMT, int W>
-__global__ __launch_bounds__(256, HDP == 32 ? (Pieces<T>::n == 2 ? 4 : 5) : HDP == 64 ? 4 : HDP == 96 ? 3 : 2) void attend_few_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int items) {
+__global__ __launch_bounds__(256, (few_waves<T, HDP, FMT, W>())) void attend_few_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j,
+                                                                                     int max_q, int items) {
     constexpr int NP = Pieces<T>::n, C64 = HDP / 64, TAIL32 = (HDP / 32) & 1, CB = HDP / 32;
     constexpr int JOIN = W == 1 ? 0 : W * (HDP * 16 + 32) * 4, TILES = 4 * 32 * HDP;
     __shared__ __attribute__((aligned(16))) char smem[JOIN > TILES ? JOIN : TILES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
-    int id = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    const int id = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
     if (W == 1 && id >= items) return;
-    const int split = id % j.splits;
-    const int item = id / j.splits;
-    const int kvh = item % j.kv_heads, t0 = item / j.kv_heads, rb = t0 % j.row_blocks, s = t0 / j.row_blocks;
-    const int* table = j.page_table + (long)s * j.max_pages;
-    int first_page = W == 1 ? table[0] : -1;                        // (asked for before the lengths are known)
-    const Span sp = span_of(j, s, max_q);
-    const int rho = rb * 16 + c16, n_rho = sp.nq * j.group;
-    if (rb * 16 >= n_rho || split * j.chunk >= max(sp.n, 1)) return;      // the whole workgroup
-    const int token = rho / j.group, head = kvh * j.group + (rho - token * j.group);
-    const bool live = rho < n_rho;
-    const long row = sp.q0 + (live ? token : 0);
-    int limit = live ? sp.n : 0;
-    if (j.visible && live) limit = max(0, min(limit, j.visible[row]));
-
-    // the split's keys that any row of the block sees, a run of whole steps for each wave
-    int most = limit;
-    if (j.visible) {
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o));
-    }
-    most = __builtin_amdgcn_readfirstlane(most);                    // (lane 0's row is there)
-    const int share = W == 1 ? j.chunk : j.chunk / W;
-    const int k_begin = split * j.chunk + (W == 1 ? 0 : wave * share), k_end = min(k_begin + share, most);
+    const int item = j.by_splits.over(id), split = id - item * j.splits;
+    const int t0 = j.by_heads.over(item), kvh = item - t0 * j.kv_heads, s = j.by_blocks.over(t0), rb = t0 - s * j.row_blocks;
+    const int share = W == 1 ? j.chunk : j.chunk / W, k_begin = split * j.chunk + (W == 1 ? 0 : wave * share);
 
     // this lane's part of a V tile: it copies 16 bytes of HDP / 32 keys
     char* vt = smem + wave * (32 * HDP);
@@ -78,22 +68,23 @@ __global__ __launch_bounds__(256, HDP == 32 ? (Pieces<T>::n == 2 ? 4 : 5) : HDP 
     const int k_off8 = min(64 * C64 + 8 * g, j.row_bytes - 8);
 
     // the pages of a step's two blocks of 16 keys (a page holds a multiple of 16 slots); a block without one reads as empty slots
-    int pi = k_begin / j.page_size, off = k_begin - pi * j.page_size;
-    auto block_row = [&](int key) -> long {
+    const int* table = j.page_table + (long)s * j.max_pages;
+    int pi = j.by_page.over(k_begin), off = k_begin - pi * j.page_size;
+    auto block_row = [&]() -> long {
         long r = -1;
-        if (key < k_end) {
-            const int page = W == 1 && pi == 0 ? first_page : table[pi];
+        if (pi < j.max_pages) {
+            const int page = table[pi];
             if (page >= 0 && page < j.pages) r = ((long)page * j.kv_heads + kvh) * j.page_size + off;
         }
         off += 16;
         if (off >= j.page_size) { off = 0; ++pi; }
         return r;
     };
-    auto fetch = [&](Step<HDP>& st, int k0) {
+    auto fetch = [&](Step<HDP>& st) {
         long r[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            r[b] = block_row(k0 + 16 * b);
+            r[b] = block_row();
             const bool any = r[b] >= 0;
             if (!any) r[b] = 0;                                     // slot 0 exists: its bytes are read and not used
             const uint8_t* kr = j.k + (r[b] + c16) * j.row_bytes;
@@ -108,17 +99,31 @@ __global__ __launch_bounds__(256, HDP == 32 ? (Pieces<T>::n == 2 ? 4 : 5) : HDP 
         for (int i = 0; i < CB; ++i)
             st.v[i] = *reinterpret_cast<const u32x4*>(j.v + ((v_key[i] < 16 ? r[0] : r[1]) + (v_key[i] & 15)) * j.row_bytes + v_col[i]);
     };
+    // the first keys are asked for before it is known whether the sequence has them (the planes hold them in any case): the loads
+    // of lengths, query rows and keys are in flight together
+    Step<HDP> even, odd;
+    fetch(even);
 
-    f32x4 o[CB][2];
+    const Span sp = span_of(j, s, max_q);
+    const int rho = rb * 16 + c16, n_rho = sp.nq * j.group;
+    if (rb * 16 >= n_rho || split * j.chunk >= max(sp.n, 1)) return;      // the whole workgroup
+    const int token = j.by_group.over(rho), head = kvh * j.group + (rho - token * j.group);
+    const bool live = rho < n_rho;
+    const long row = sp.q0 + (live ? token : 0);
+    // what a row sees ends at `limit`; most: what any row of the block sees
+    int limit = sp.n, most = sp.n;
+    if (j.visible) {
+        limit = most = live ? max(0, min(sp.n, j.visible[row])) : 0;
 #pragma unroll
-    for (int i = 0; i < CB; ++i) { o[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; o[i][1] = o[i][0]; }
-    float m_run = LOWEST, l_run = 0.f;
-    int v_ref = 1;                                                  // largest exponent byte of V so far, the same in every lane
+        for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o));
+        if (!live) limit = most;                                    // (rows that are not there take no part in the tests below)
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    const int k_end = min(k_begin + share, most);
+    limit = min(limit, k_end);
 
-    Step<HDP> now, next;
-    if (k_begin < k_end) fetch(now, k_begin);                       // in flight while q is brought into shape
     f16x8 qf[2 * C64 + TAIL32][NP];
-    float c_row;
+    float c_row;                                                    // from products of halves to octaves, not negative
     {
         float f[2 * C64 + TAIL32][8], amax = 0.f;
         const T* qr = q + row * j.ldq + (long)head * j.hd;
@@ -127,21 +132,31 @@ __global__ __launch_bounds__(256, HDP == 32 ? (Pieces<T>::n == 2 ? 4 : 5) : HDP 
             const int e = i < 2 * C64 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 64 * C64 + 8 * g;
             query8<T>(qr + e, live && e < j.hd, f[i]);
 #pragma unroll
-            for (int x = 0; x < 8; ++x) amax = fmaxf(amax, fabsf(f[i][x]));
+            for (int x = 0; x < 8; ++x) {
+                amax = fmaxf(amax, fabsf(f[i][x]));
+                f[i][x] = copysignf(1.f, j.scale_log2e) * f[i][x];
+            }
         }
         amax = fmaxf(amax, __shfl_xor(amax, 16));
         amax = fmaxf(amax, __shfl_xor(amax, 32));
         const int shift = query_shift(amax);
 #pragma unroll
         for (int i = 0; i < 2 * C64 + TAIL32; ++i) query_pieces<NP>(f[i], shift, qf[i]);
-        c_row = __builtin_amdgcn_ldexpf(j.scale_log2e, -shift);
+        c_row = fmaxf(__builtin_amdgcn_ldexpf(fabsf(j.scale_log2e), -shift), 1e-36f);      // (0 times -infinity is no score)
     }
 
-    for (int k0 = k_begin; k0 < k_end; k0 += 32) {
-        if (k0 + 32 < k_end) fetch(next, k0 + 32);
+    f32x4 o[CB][2];
+#pragma unroll
+    for (int i = 0; i < CB; ++i) { o[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; o[i][1] = o[i][0]; }
+    // m_run: largest score so far in octaves.  Values' exponents are relative to v_ref, the largest so far (the same in every lane):
+    // probabilities, their sum and the outputs all carry the factor 2^(127 + P_SHIFT - v_ref), which cancels in the end
+    float m_run = LOWEST, l_run = 0.f;
+    int v_ref = V_REF_MIN;
+
+    auto step = [&](Step<HDP>& st, int k0) {
         // V codes to LDS (in the order of the keys); the wave alone reads them, LDS operations of a wave stay in order
 #pragma unroll
-        for (int i = 0; i < CB; ++i) *reinterpret_cast<u32x4*>(vt + v_lds[i]) = now.v[i];
+        for (int i = 0; i < CB; ++i) *reinterpret_cast<u32x4*>(vt + v_lds[i]) = st.v[i];
         asm volatile("" ::: "memory");
 
         float sc[2][4];
@@ -152,72 +167,72 @@ __global__ __launch_bounds__(256, HDP == 32 ? (Pieces<T>::n == 2 ? 4 : 5) : HDP 
             for (int i = 0; i < C64; ++i)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const f16x8 kf = codes8<FMT>(u32x2{now.k[b][i][2 * h], now.k[b][i][2 * h + 1]});
+                    const f16x8 kf = codes8<FMT>(u32x2{st.k[b][i][2 * h], st.k[b][i][2 * h + 1]});
 #pragma unroll
                     for (int p = NP - 1; p >= 0; --p) a = mfma16(kf, qf[2 * i + h][p], a);
                 }
             if (TAIL32) {
-                const f16x8 kf = codes8<FMT>(now.k8[b]);
+                const f16x8 kf = codes8<FMT>(st.k8[b]);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p) a = mfma16(kf, qf[2 * C64][p], a);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[b][i] = a[i] * (c_row * power_of_byte(byte_of(now.ek[b], i)));
+            for (int i = 0; i < 4; ++i) sc[b][i] = a[i] * power_of_byte(byte_of(st.ek[b], i));
         }
+        int top = 0;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max(top, (int)byte_of(st.ev[b], i));
         // what is not seen: keys beyond the row's limit, empty slots; what is seen and not a number: rows with exponent 255
         unsigned keep[2] = {0xffffffffu, 0xffffffffu};
-        const unsigned odd = zero_bytes(now.ek[0]) | zero_bytes(now.ek[1]) | zero_bytes(~now.ek[0]) | zero_bytes(~now.ek[1]) | zero_bytes(~now.ev[0]) | zero_bytes(~now.ev[1]);
-        if (__builtin_amdgcn_ballot_w64(odd != 0 || k0 + 32 > limit || k0 + 32 > k_end) != 0) {
+        if (__builtin_amdgcn_ballot_w64((odd_bytes(st.ek[0]) | odd_bytes(st.ek[1])) != 0 || top == 255 || k0 + 32 > limit) != 0) {
+            top = 0;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 keep[b] = 0u;
                 unsigned ev = 0u;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int key = k0 + 16 * b + 4 * g + i, e = byte_of(now.ek[b], i), w = byte_of(now.ev[b], i);
-                    const bool nan = e == 255 || w == 255;
-                    if (key >= k_end || e == 0) {
-                        sc[b][i] = -INFINITY;
-                    } else if (nan) {
-                        sc[b][i] = key < limit ? __builtin_nanf("") : -INFINITY;
-                    } else {
+                    const int key = k0 + 16 * b + 4 * g + i;
+                    const unsigned e = byte_of(st.ek[b], i), w = byte_of(st.ev[b], i);
+                    const bool there = key < k_end && e != 0, nan = e == 255 || w == 255;
+                    if (there && !nan) {
                         keep[b] |= 255u << (8 * i);
-                        ev |= (unsigned)w << (8 * i);
-                        if (key >= limit) sc[b][i] = -INFINITY;
+                        ev |= w << (8 * i);
+                        top = max(top, (int)w);
                     }
+                    if (!there || key >= limit) sc[b][i] = -INFINITY;
+                    else if (nan) sc[b][i] = __builtin_nanf("");
                 }
-                now.ev[b] = ev;
+                st.ev[b] = ev;
             }
         }
-        float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-        int ve[2][4], top = 0;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { ve[b][i] = byte_of(now.ev[b], i); top = max(top, ve[b][i]); }
+        float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * c_row;
         if (__builtin_amdgcn_ballot_w64(mx > m_run + DEFER || top > v_ref) != 0) {
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             top = max(top, __shfl_xor(top, 16));
             top = max(top, __shfl_xor(top, 32));
-            const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            const float m_new = fmaxf(m_run, mx);
             const int ref = max(v_ref, top);
-            const float beta = __builtin_amdgcn_ldexpf(alpha, v_ref - ref);
+            const float alpha = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(m_run - m_new), v_ref - ref);
             l_run *= alpha;
 #pragma unroll
-            for (int i = 0; i < CB; ++i) { o[i][0] *= beta; o[i][1] *= beta; }
+            for (int i = 0; i < CB; ++i) { o[i][0] *= alpha; o[i][1] *= alpha; }
             m_run = m_new;
             v_ref = ref;
         }
+        const float base = (float)(127 + P_SHIFT - v_ref) - m_run;
         f16x8 pf[NP];
         float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(sc[b][i] - m_run);
+                const float p = __builtin_amdgcn_exp2f(fmaf(sc[b][i], c_row, base));
                 sum += p;
-                const float w = __builtin_amdgcn_ldexpf(p, ve[b][i] - v_ref + P_SHIFT);
+                const float w = p * power_of_byte(byte_of(st.ev[b], i));
                 const f16 hi = (f16)w;
                 pf[0][4 * b + i] = hi;
                 if (NP == 2) pf[NP - 1][4 * b + i] = (f16)(w - (float)hi);
@@ -233,25 +248,36 @@ __global__ __launch_bounds__(256, HDP == 32 ? (Pieces<T>::n == 2 ? 4 : 5) : HDP 
 #pragma unroll
             for (int par = 0; par < 2; ++par) {
                 const unsigned sel = par ? 0x07050301u : 0x06040200u;
-                const u32x2 w = {__builtin_amdgcn_perm(r0[1], r0[0], sel) & keep[0], __builtin_amdgcn_perm(r1[1], r1[0], sel) & keep[1]};
+                u32x2 w = {__builtin_amdgcn_perm(r0[1], r0[0], sel), __builtin_amdgcn_perm(r1[1], r1[0], sel)};
+                if (FMT == VDA_CACHE_E4M3) { w[0] &= keep[0]; w[1] &= keep[1]; }
                 const f16x8 vf = codes8<FMT>(w);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p) o[i][par] = mfma16(vf, pf[p], o[i][par]);
             }
         }
-        now = next;
+    };
+    for (int k0 = k_begin; k0 < k_end; k0 += 64) {
+        if (k0 + 32 < k_end) fetch(odd);
+        step(even, k0);
+        if (k0 + 32 >= k_end) break;
+        if (k0 + 64 < k_end) fetch(even);
+        step(odd, k0 + 32);
     }
 
     // lane (c16, g) holds channels 32 i + 8 g + 0..7 of query c16, even ones in o[i][0], odd ones in o[i][1]
     l_run += __shfl_xor(l_run, 16);
     l_run += __shfl_xor(l_run, 32);
+    if (W > 1 || j.splits > 1) {         // parts with references of their own will meet: back to their own scale
+        const int back = v_ref - 127 - P_SHIFT;
+        l_run = __builtin_amdgcn_ldexpf(l_run, back);
 #pragma unroll
-    for (int i = 0; i < CB; ++i)
+        for (int i = 0; i < CB; ++i)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            o[i][0][x] = __builtin_amdgcn_ldexpf(o[i][0][x], v_ref - 127 - P_SHIFT);
-            o[i][1][x] = __builtin_amdgcn_ldexpf(o[i][1][x], v_ref - 127 - P_SHIFT);
-        }
+            for (int x = 0; x < 4; ++x) {
+                o[i][0][x] = __builtin_amdgcn_ldexpf(o[i][0][x], back);
+                o[i][1][x] = __builtin_amdgcn_ldexpf(o[i][1][x], back);
+            }
+    }
     if (W > 1) {        // join the waves' parts: [wave][16 rows][HDP] outputs, then [wave][16] maxima and sums
         __syncthreads();                                            // the V tiles are done with
         float* jo = reinterpret_cast<float*>(smem);
@@ -288,13 +314,13 @@ __global__ __launch_bounds__(256, HDP == 32 ? (Pieces<T>::n == 2 ? 4 : 5) : HDP 
     if (!live) return;
     if (j.splits > 1) {
         float* p = j.part + ((long)item * j.splits + split) * (16 * (HDP + 2));
+        if (g == 0) { p[16 * HDP + c16] = m_run; p[16 * HDP + 16 + c16] = l_run; }
 #pragma unroll
         for (int i = 0; i < CB; ++i) {
             float* d = p + c16 * HDP + 32 * i + 8 * g;
             *reinterpret_cast<f32x4*>(d) = f32x4{o[i][0][0], o[i][1][0], o[i][0][1], o[i][1][1]};
             *reinterpret_cast<f32x4*>(d + 4) = f32x4{o[i][0][2], o[i][1][2], o[i][0][3], o[i][1][3]};
         }
-        if (g == 0) { p[16 * HDP + c16] = m_run; p[16 * HDP + 16 + c16] = l_run; }
         return;
     }
     const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
@@ -314,7 +340,7 @@ __global__ __launch_bounds__(256, HDP == 32 ? (Pieces<T>::n == 2 ? 4 : 5) : HDP 
 // A thread per row and four channels; grid (item, run of rows).
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(T* __restrict__ out, AttendJob j, int max_q, int block_rows, int hdp) {
-    const int item = blockIdx.x, kvh = item % j.kv_heads, t0 = item / j.kv_heads, rb = t0 % j.row_blocks, s = t0 / j.row_blocks;
+    const int item = blockIdx.x, t0 = j.by_heads.over(item), kvh = item - t0 * j.kv_heads, s = j.by_blocks.over(t0), rb = t0 - s * j.row_blocks;
     const Span sp = span_of(j, s, max_q);
     const int rows = min(block_rows, sp.nq * j.group - rb * block_rows), quads = j.hd / 4, per = 256 / quads;
     const int r0 = threadIdx.x / quads, r = blockIdx.y * per + r0, d = (threadIdx.x - r0 * quads) * 4;
@@ -336,7 +362,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(T* __restrict__ out, A
         o = a * o + b * ox;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int rho = rb * block_rows + r, token = rho / j.group;
+    const int rho = rb * block_rows + r, token = j.by_group.over(rho);
     const typename Vec<T>::v4 y = {(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
     *reinterpret_cast<typename Vec<T>::v4*>(out + (sp.q0 + token) * j.ldo + (long)(kvh * j.group + rho - token * j.group) * j.hd + d) = y;
 }

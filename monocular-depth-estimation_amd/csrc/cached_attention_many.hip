@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
             const u32x4 e = *reinterpret_cast<const u32x4*>(j.k_exp + at), w = *reinterpret_cast<const u32x4*>(j.v_exp + at);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int be = byte_of(e[i >> 2], i & 3), bw = byte_of(w[i >> 2], i & 3);
+                const int be = (int)byte_of(e[i >> 2], i & 3), bw = (int)byte_of(w[i >> 2], i & 3);
                 if (key + i < k_end && be != 0 && be != 255 && bw != 255) { tk = max(tk, be); tv = max(tv, bw); }
             }
         }

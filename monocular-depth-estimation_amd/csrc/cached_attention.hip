@@ -14,7 +14,7 @@ struct Plan {
 // are fewer, four waves share an item and the key axis is split over workgroups, down to 128 keys for each wave.
 // More rows: the kernel whose workgroups of 128 rows share decoded tiles; the key axis is split, down to 512 keys, until the
 // workgroups that a CU holds at once (three, two for wide heads) are there.
-constexpr int FEW_ROWS = 32, MIN_FEW = 256, MIN_MANY = 512;
+constexpr int FEW_ROWS = 32, ONE_FEW = 2048, MIN_FEW = 512, MIN_MANY = 512;
 int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int heads, Plan* p) {
     if (const int rc = cache_check(c)) return rc;
     if (seqs <= 0 || max_pages <= 0 || max_q <= 0 || heads <= 0) return VDA_EINVAL;
@@ -25,11 +25,10 @@ int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int head
     p->hd_pad = (c->hd + 31) & ~31;
     const long blocks = (rows + p->block_rows - 1) / p->block_rows, items = blocks * seqs * c->kv_heads;
     if (rows > 0x7fffffffL || items > 0x3fffffffL) return VDA_ESHAPE;
-    // keys of a part: in few-row calls a multiple of 128 (32 for each of four waves), else of 64
-    long chunk = keys;
+    long chunk = keys;                                            // keys of a part: 32 for each of eight waves, or more
     if (few) {
-        p->waves = items >= 4096 || keys <= 64 ? 1 : 4;
-        if (p->waves == 4) {
+        p->waves = items >= 4096 || keys <= 64 ? 1 : 8;
+        if (p->waves == 8 && keys > ONE_FEW) {
             const long wanted = 2048 / items;                     // parts, if there are keys enough
             chunk = wanted <= 1 ? keys : (keys + wanted - 1) / wanted;
             chunk = chunk < MIN_FEW ? MIN_FEW : chunk;
@@ -40,7 +39,7 @@ int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int head
         chunk = wanted <= 1 ? keys : (keys + wanted - 1) / wanted;
         chunk = chunk < MIN_MANY ? MIN_MANY : chunk;
     }
-    chunk = (chunk + 127) & ~127L;
+    chunk = (chunk + 255) & ~255L;
     if (chunk > 0x40000000L) return VDA_ESHAPE;
     const long splits = (keys + chunk - 1) / chunk;
     p->chunk = (int)chunk;

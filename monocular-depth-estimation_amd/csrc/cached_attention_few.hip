@@ -33,7 +33,7 @@ template <int HDP> struct Step {
 };
 
 // Waves per SIMD that the registers allow without spilling (32, 64, 96, 128 channels; more pieces of q or the longer code of W = 1
-// cost one).
+// cost one).  A workgroup of W = 8 has two on each SIMD.
 template <typename T, int HDP, int FMT, int W> constexpr int few_waves() {
     constexpr bool big = Pieces<T>::n == 2 || (W == 1 && (HDP > 32 || FMT == VDA_CACHE_E4M3));
     return HDP == 32 ? (big ? 4 : 5) : HDP == 64 ? (big ? 3 : 4) : HDP == 96 ? (big ? 2 : 3) : 2;
@@ -41,10 +41,10 @@ template <typename T, int HDP, int FMT, int W> constexpr int few_waves() {
 
 // W waves share a (sequence, key head, row block, split) item, each with a part of its keys; W = 1: a wave per item.
 template <typename T, int HDP, int FMT, int W>
-__global__ __launch_bounds__(256, (few_waves<T, HDP, FMT, W>())) void attend_few_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j,
-                                                                                     int max_q, int items) {
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP, FMT, W>())) void attend_few_kernel(const T* __restrict__ q, T* __restrict__ out,
+                                                                                                       AttendJob j, int max_q, int items) {
     constexpr int NP = Pieces<T>::n, C64 = HDP / 64, TAIL32 = (HDP / 32) & 1, CB = HDP / 32;
-    constexpr int JOIN = W == 1 ? 0 : W * (HDP * 16 + 32) * 4, TILES = 4 * 32 * HDP;
+    constexpr int LD = HDP + 4, JOIN = W == 1 ? 0 : W * (LD * 16 + 32) * 4, TILES = (W == 1 ? 4 : W) * 32 * HDP;
     __shared__ __attribute__((aligned(16))) char smem[JOIN > TILES ? JOIN : TILES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, FMT, W>())) void attend_few
     // lane (c16, g) holds channels 32 i + 8 g + 0..7 of query c16, even ones in o[i][0], odd ones in o[i][1]
     l_run += __shfl_xor(l_run, 16);
     l_run += __shfl_xor(l_run, 32);
-    if (W > 1 || j.splits > 1) {         // parts with references of their own will meet: back to their own scale
+    if (W > 1) {         // parts with references of their own will meet: back to their own scale
         const int back = v_ref - 127 - P_SHIFT;
         l_run = __builtin_amdgcn_ldexpf(l_run, back);
 #pragma unroll
@@ -278,61 +278,55 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, FMT, W>())) void attend_few
                 o[i][1][x] = __builtin_amdgcn_ldexpf(o[i][1][x], back);
             }
     }
-    if (W > 1) {        // join the waves' parts: [wave][16 rows][HDP] outputs, then [wave][16] maxima and sums
+    if constexpr (W > 1) {        // join the waves' parts: [wave][16 rows][LD] outputs, then [wave][16] maxima and sums
         __syncthreads();                                            // the V tiles are done with
         float* jo = reinterpret_cast<float*>(smem);
-        float* jm = jo + W * 16 * HDP;
+        float* jm = jo + W * 16 * LD;
 #pragma unroll
         for (int i = 0; i < CB; ++i) {
-            float* p = jo + (wave * 16 + c16) * HDP + 32 * i + 8 * g;
+            float* p = jo + (wave * 16 + c16) * LD + 32 * i + 8 * g;
             *reinterpret_cast<f32x4*>(p) = f32x4{o[i][0][0], o[i][1][0], o[i][0][1], o[i][1][1]};
             *reinterpret_cast<f32x4*>(p + 4) = f32x4{o[i][0][2], o[i][1][2], o[i][0][3], o[i][1][3]};
         }
         if (g == 0) { jm[wave * 16 + c16] = m_run; jm[W * 16 + wave * 16 + c16] = l_run; }
         __syncthreads();
-        if (wave != 0) return;
-        float m = LOWEST;
+        float* part = j.part + ((long)item * j.splits + split) * (16 * (HDP + 2));
+        for (int x = threadIdx.x; x < 16 * (HDP / 4); x += 64 * W) {       // a row and four channels per thread
+            const int r = x / (HDP / 4), d = (x % (HDP / 4)) * 4, rho_r = rb * 16 + r;
+            if (rho_r >= n_rho) continue;
+            float m = LOWEST, l = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) m = fmaxf(m, jm[w * 16 + c16]);
-        l_run = 0.f;
+            for (int w = 0; w < W; ++w) m = fmaxf(m, jm[w * 16 + r]);
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < CB; ++i) { o[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; o[i][1] = o[i][0]; }
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float a = __builtin_amdgcn_exp2f(jm[w * 16 + c16] - m);
-            l_run += a * jm[W * 16 + w * 16 + c16];
-#pragma unroll
-            for (int i = 0; i < CB; ++i) {
-                const float* p = jo + (w * 16 + c16) * HDP + 32 * i + 8 * g;
-                const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
-                o[i][0] += a * f32x4{x[0], x[2], y[0], y[2]};
-                o[i][1] += a * f32x4{x[1], x[3], y[1], y[3]};
+            for (int w = 0; w < W; ++w) {
+                const float a = __builtin_amdgcn_exp2f(jm[w * 16 + r] - m);
+                l += a * jm[W * 16 + w * 16 + r];
+                v += a * *reinterpret_cast<const f32x4*>(jo + (w * 16 + r) * LD + d);
+            }
+            if (j.splits > 1) {
+                *reinterpret_cast<f32x4*>(part + r * HDP + d) = v;
+                if (d == 0) { part[16 * HDP + r] = m; part[16 * HDP + 16 + r] = l; }
+            } else if (d < j.hd) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const int tok = j.by_group.over(rho_r);
+                const typename Vec<T>::v4 y = {(T)(v[0] * inv), (T)(v[1] * inv), (T)(v[2] * inv), (T)(v[3] * inv)};
+                *reinterpret_cast<typename Vec<T>::v4*>(out + (sp.q0 + tok) * j.ldo + (long)(kvh * j.group + rho_r - tok * j.group) * j.hd + d) = y;
             }
         }
-        m_run = m;
-    }
-    if (!live) return;
-    if (j.splits > 1) {
-        float* p = j.part + ((long)item * j.splits + split) * (16 * (HDP + 2));
-        if (g == 0) { p[16 * HDP + c16] = m_run; p[16 * HDP + 16 + c16] = l_run; }
+    } else {
+        if (!live) return;
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        T* orow = out + row * j.ldo + (long)head * j.hd;
 #pragma unroll
         for (int i = 0; i < CB; ++i) {
-            float* d = p + c16 * HDP + 32 * i + 8 * g;
-            *reinterpret_cast<f32x4*>(d) = f32x4{o[i][0][0], o[i][1][0], o[i][0][1], o[i][1][1]};
-            *reinterpret_cast<f32x4*>(d + 4) = f32x4{o[i][0][2], o[i][1][2], o[i][0][3], o[i][1][3]};
+            const int d = 32 * i + 8 * g;
+            if (d >= j.hd) continue;
+            typename Vec<T>::v8 r;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) { r[2 * x] = (T)(o[i][0][x] * inv); r[2 * x + 1] = (T)(o[i][1][x] * inv); }
+            *reinterpret_cast<typename Vec<T>::v8*>(orow + d) = r;
         }
-        return;
-    }
-    const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-    T* orow = out + row * j.ldo + (long)head * j.hd;
-#pragma unroll
-    for (int i = 0; i < CB; ++i) {
-        const int d = 32 * i + 8 * g;
-        if (d >= j.hd) continue;
-        typename Vec<T>::v8 r;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) { r[2 * x] = (T)(o[i][0][x] * inv); r[2 * x + 1] = (T)(o[i][1][x] * inv); }
-        *reinterpret_cast<typename Vec<T>::v8*>(orow + d) = r;
     }
 }
 
@@ -371,8 +365,8 @@ template <typename T>
 int few(const AttendJob& j, const T* q, T* out, int format, int max_q, int waves, hipStream_t st) {
     const int items = j.seqs * j.kv_heads * j.row_blocks * j.splits;
     const int grid = waves == 1 ? (items + 3) / 4 : items;
-#define VDA_F3(H, F, W) hipLaunchKernelGGL((attend_few_kernel<T, H, F, W>), dim3(grid), dim3(256), 0, st, q, out, j, max_q, items)
-#define VDA_F2(H, F) do { if (waves == 1) VDA_F3(H, F, 1); else VDA_F3(H, F, 4); } while (0)
+#define VDA_F3(H, F, W) hipLaunchKernelGGL((attend_few_kernel<T, H, F, W>), dim3(grid), dim3(W == 1 ? 256 : 64 * W), 0, st, q, out, j, max_q, items)
+#define VDA_F2(H, F) do { if (waves == 1) VDA_F3(H, F, 1); else VDA_F3(H, F, 8); } while (0)
 #define VDA_F(H) do { if (format == VDA_CACHE_I8) VDA_F2(H, VDA_CACHE_I8); else VDA_F2(H, VDA_CACHE_E4M3); } while (0)
     if (j.hd <= 32) VDA_F(32);
     else if (j.hd <= 64) VDA_F(64);

@@ -9,18 +9,22 @@ struct Plan {
     long work;
 };
 
-// Up to 32 rows per key head: the kernel whose waves hold 16 rows each and read the cache straight into registers.  It wants
+// Up to 32 rows per key head, or few rows of work in all (blocks of 16 rows times keys): the kernel whose waves hold 16 rows each and read the cache straight into registers.  It wants
 // enough waves in flight to draw the full memory bandwidth, a few thousand: where the (sequence, key head, row block) items alone
 // are fewer, four waves share an item and the key axis is split over workgroups, down to 128 keys for each wave.
 // More rows: the kernel whose workgroups of 128 rows share decoded tiles; the key axis is split, down to 512 keys, until the
 // workgroups that a CU holds at once (three, two for wide heads) are there.
-constexpr int FEW_ROWS = 32, ONE_FEW = 2048, MIN_FEW = 512, MIN_MANY = 512;
+// Measured, 8 heads of 64, us of this kernel / the other: 32 rows over 16384 keys 31 / 30, 64 rows 38 / 30; 384 rows over 2048 keys
+// 17 / 24; 8 sequences of 64 rows over 2048 keys 17 / 25, of 192 rows 34 / 36, of 384 rows 60 / 43.
+constexpr int FEW_ROWS = 32, FEW_KEYS = 4096, FEW_WORK = 3 << 18;
+constexpr int ONE_FEW = 2048, MIN_FEW = 512, MIN_MANY = 512;
 int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int heads, Plan* p) {
     if (const int rc = cache_check(c)) return rc;
     if (seqs <= 0 || max_pages <= 0 || max_q <= 0 || heads <= 0) return VDA_EINVAL;
     if (heads % c->kv_heads != 0 || (long)max_pages * c->page_size > 0x7fffffffL) return VDA_ESHAPE;
     const long rows = (long)max_q * (heads / c->kv_heads), keys = (long)max_pages * c->page_size;
-    const bool few = rows <= FEW_ROWS;
+    const long few_items = (rows + 15) / 16 * seqs * c->kv_heads;
+    const bool few = rows <= FEW_ROWS || (keys <= FEW_KEYS && few_items <= FEW_WORK / keys);
     p->block_rows = few ? 16 : 128;
     p->hd_pad = (c->hd + 31) & ~31;
     const long blocks = (rows + p->block_rows - 1) / p->block_rows, items = blocks * seqs * c->kv_heads;

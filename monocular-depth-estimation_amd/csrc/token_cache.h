@@ -13,3 +13,17 @@ static inline int cache_check(const VdaTokenCache* c) {
     if ((long)c->pages * c->page_size > 0x7fffffffL || (long)c->pages * c->page_size * c->kv_heads > (1L << 40)) return VDA_ESHAPE;
     return VDA_OK;
 }
+
+// n / d for 0 <= n < 2^31 and a divisor known when the call is made: one high product and a shift.  With l = ceil(log2 d) and
+// m = ceil(2^(31 + l) / d) the product n m / 2^(31 + l) exceeds n / d by less than n / 2^31 < 1 of 1 / d, which reaches no next integer.
+struct Quick {
+    unsigned d, m;
+    int s;
+    explicit Quick(unsigned n) : d(n) {
+        int l = 0;
+        while ((1ull << l) < n) ++l;
+        m = (unsigned)(((1ull << (31 + l)) + n - 1) / n);
+        s = l - 1;
+    }
+    __device__ __forceinline__ int over(int n) const { return d == 1 ? n : (int)(__umulhi((unsigned)n, m) >> s); }
+};

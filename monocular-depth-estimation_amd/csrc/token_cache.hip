@@ -11,6 +11,7 @@ struct Axes {
     const void* pos;
     const double* freq;
     int half, end_t, end_h, pos_float;
+    Quick by_half;
 };
 __device__ __forceinline__ float2 turn(const Axes& a, long row, int j) {
     const int axis = j < a.end_t ? 0 : j < a.end_h ? 1 : 2;
@@ -38,56 +39,123 @@ __device__ __forceinline__ void store_f32(T* p, const float* f) {
     *reinterpret_cast<Pack<T, N>*>(p) = r;
 }
 
-// A workgroup turns `tb` tokens: first the angles of their tb * half pairs into LDS, then one unit of U pairs per thread.  A
-// thread holds both members of its pairs, so the call may be in place.
-template <typename T, int U, bool ADJ>
-__global__ __launch_bounds__(256) void rotary_kernel(const T* x, T* out, Axes ax, long rows, long ldx, long ldo, int heads, int hd, int tb,
-                                                     int copies) {
-    extern __shared__ float2 cs[];
-    const long r0 = (long)blockIdx.x * tb;
-    const int nt = (int)min((long)tb, rows - r0);
-    const int half = ax.half;
-    for (int i = threadIdx.x; i < nt * half; i += 256) {
-        const int t = i / half;
-        cs[i] = turn(ax, r0 + t, i - t * half);
+// A workgroup turns `tb` tokens: first the angles of their tb * half pairs into LDS, then the rows, each thread keeping one piece of the
+// row (or several 256 apart) and walking down the tokens, so that no address is divided out.
+struct RotaryShape {
+    long rows, ldx, ldo;
+    int heads, hd, tb, per_head, far;       // pieces of a head; line form: lanes between the two channels of a pair
+    Quick by_row, by_head;                  // pieces of a row, of a head
+};
+struct Walk {
+    int piece, t, side;                     // first piece of this thread, first token, tokens side by side
+};
+__device__ __forceinline__ bool walk(const RotaryShape& s, Walk& w) {
+    const int per_row = s.heads * s.per_head, tid = threadIdx.x;
+    w = Walk{tid, 0, 1};
+    if (per_row < 256) {
+        w.side = s.by_row.over(256);
+        w.t = s.by_row.over(tid);
+        w.piece = tid - w.t * per_row;
+    }
+    return w.t < w.side;
+}
+__device__ __forceinline__ void angles(float2* cs, const Axes& ax, long r0, int nt) {
+    for (int i = threadIdx.x; i < nt * ax.half; i += 256) {
+        const int t = ax.by_half.over(i);
+        cs[i] = turn(ax, r0 + t, i - t * ax.half);
     }
     __syncthreads();
-    constexpr int CU = U < 4 ? 4 : (sizeof(T) == 2 ? 8 : 4);         // channels of a unit that is only copied
-    const unsigned units = half / U, per_head = units + copies, per_row = per_head * heads;
-    for (unsigned i = threadIdx.x; i < nt * per_row; i += 256) {
-        const unsigned t = i / per_row, in_row = i - t * per_row, head = in_row / per_head, u = in_row - head * per_head;
-        const T* xr = x + (r0 + t) * ldx + head * hd;
-        T* yr = out + (r0 + t) * ldo + head * hd;
-        if (u >= units) {
-            float f[CU];
-            const int c = 2 * half + (u - units) * CU;
-            load_f32<T, CU>(xr + c, f);
-            store_f32<T, CU>(yr + c, f);
-            continue;
+}
+
+// Line form: a lane moves 16 bytes of the row, neighbours moving neighbouring ones, and takes the other channels of its pairs from the
+// lane `far` away (a power of two: both lie in one group of 2 far lanes, which hold one head's pieces or a part of them).  Reading
+// both halves of a head in one thread instead touches every cache line twice, by halves: 101 against 75 us for q and k of 32
+// frames of 1370 tokens (16 heads of 64, 16-bit, 359 MB moved: 4.8 TB/s).  All lanes of a group load before any of them stores: the call may be in place.
+template <typename T, bool ADJ>
+__global__ __launch_bounds__(256) void rotary_line_kernel(const T* x, T* out, Axes ax, RotaryShape s) {
+    extern __shared__ float2 cs[];
+    constexpr int N = 16 / sizeof(T);
+    const long r0 = (long)blockIdx.x * s.tb;
+    const int nt = (int)min((long)s.tb, s.rows - r0), half = ax.half;
+    angles(cs, ax, r0, nt);
+    Walk w;
+    if (!walk(s, w)) return;
+    for (int c = w.piece; c < s.heads * s.per_head; c += 256) {
+        const int head = s.by_head.over(c), e0 = (c - head * s.per_head) * N;                   // first channel of the piece in its head
+        const bool turned = e0 < 2 * half, second = e0 >= half;
+        const T* xr = x + (r0 + w.t) * s.ldx + (long)c * N;
+        T* yr = out + (r0 + w.t) * s.ldo + (long)c * N;
+        const float2* a = cs + w.t * half + (ADJ ? e0 >> 1 : second ? e0 - half : e0);
+        for (int t = w.t; t < nt; t += w.side) {
+            const Pack<T, N> own = *reinterpret_cast<const Pack<T, N>*>(xr);
+            Pack<T, N> res = own;
+            if constexpr (ADJ) {
+                if (turned) {
+#pragma unroll
+                    for (int k = 0; k < N; k += 2) {
+                        const float p = (float)own.v[k], q = (float)own.v[k + 1];
+                        res.v[k] = (T)(p * a[k >> 1].x - q * a[k >> 1].y);
+                        res.v[k + 1] = (T)(q * a[k >> 1].x + p * a[k >> 1].y);
+                    }
+                }
+            } else {
+                const u32x4 mine = __builtin_bit_cast(u32x4, own);
+                u32x4 their;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) their[k] = (unsigned)__shfl_xor((int)mine[k], s.far);
+                const Pack<T, N> other = __builtin_bit_cast(Pack<T, N>, their);
+                if (turned) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const float p = (float)own.v[k], q = (float)other.v[k];
+                        res.v[k] = (T)(p * a[k].x + (second ? q : -q) * a[k].y);
+                    }
+                }
+            }
+            *reinterpret_cast<Pack<T, N>*>(yr) = res;
+            xr += w.side * s.ldx;
+            yr += w.side * s.ldo;
+            a += w.side * half;
         }
-        const float2* w = cs + t * half + u * U;
-        if (ADJ) {
-            float f[2 * U], g[2 * U];
-            load_f32<T, U>(xr + 2 * U * u, f);
-            load_f32<T, U>(xr + 2 * U * u + U, f + U);
+    }
+}
+
+// The general form, for pairs in halves whose distance is no power of two pieces, and rows that are only 8-byte aligned: a
+// thread holds four pairs, or CU channels that are only copied.
+template <typename T>
+__global__ __launch_bounds__(256) void rotary_pairs_kernel(const T* x, T* out, Axes ax, RotaryShape s) {
+    extern __shared__ float2 cs[];
+    constexpr int CU = sizeof(T) == 2 ? 8 : 4;
+    const long r0 = (long)blockIdx.x * s.tb;
+    const int nt = (int)min((long)s.tb, s.rows - r0), half = ax.half, units = half / 4;
+    angles(cs, ax, r0, nt);
+    Walk w;
+    if (!walk(s, w)) return;
+    for (int c = w.piece; c < s.heads * s.per_head; c += 256) {
+        const int head = s.by_head.over(c), u = c - head * s.per_head;
+        const bool copy = u >= units;
+        const int at = head * s.hd + (copy ? 2 * half + (u - units) * CU : 4 * u);
+        const T* xr = x + (r0 + w.t) * s.ldx + at;
+        T* yr = out + (r0 + w.t) * s.ldo + at;
+        const float2* a = cs + w.t * half + 4 * u;
+        for (int t = w.t; t < nt; t += w.side) {
+            if (copy) {
+                *reinterpret_cast<Pack<T, CU>*>(yr) = *reinterpret_cast<const Pack<T, CU>*>(xr);
+            } else {
+                float p[4], q[4], y[4], z[4];
+                load_f32<T, 4>(xr, p);
+                load_f32<T, 4>(xr + half, q);
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                g[2 * k] = f[2 * k] * w[k].x - f[2 * k + 1] * w[k].y;
-                g[2 * k + 1] = f[2 * k + 1] * w[k].x + f[2 * k] * w[k].y;
+                for (int k = 0; k < 4; ++k) {
+                    y[k] = p[k] * a[k].x - q[k] * a[k].y;
+                    z[k] = q[k] * a[k].x + p[k] * a[k].y;
+                }
+                store_f32<T, 4>(yr, y);
+                store_f32<T, 4>(yr + half, z);
             }
-            store_f32<T, U>(yr + 2 * U * u, g);
-            store_f32<T, U>(yr + 2 * U * u + U, g + U);
-        } else {
-            float a[U], b[U], c[U], d[U];
-            load_f32<T, U>(xr + U * u, a);
-            load_f32<T, U>(xr + half + U * u, b);
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                c[k] = a[k] * w[k].x - b[k] * w[k].y;
-                d[k] = b[k] * w[k].x + a[k] * w[k].y;
-            }
-            store_f32<T, U>(yr + U * u, c);
-            store_f32<T, U>(yr + half + U * u, d);
+            xr += w.side * s.ldx;
+            yr += w.side * s.ldo;
+            a += w.side * half;
         }
     }
 }
@@ -104,42 +172,43 @@ __device__ __forceinline__ int exponent_byte(unsigned amax_bits, int format) {
     return max(1, min(254, e));                                    // 0 marks an empty slot
 }
 __device__ __forceinline__ u32x2 encode8(const float* f, int byte, int format) {
-    float y[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = __builtin_amdgcn_ldexpf(f[k], 127 - byte);
     u32x2 c = {0u, 0u};
     if (byte == 255) return c;
+    const float s = byte == 254 ? __uint_as_float(1u << 22) : __uint_as_float((unsigned)(254 - byte) << 23);      // 2^(127 - byte)
     if (format == VDA_CACHE_I8) {
+        // on 1.5 * 2^23 a unit in the last place is 1: the sum's one rounding, to nearest even, leaves the code in the low byte
 #pragma unroll
-        for (int k = 0; k < 8; ++k) c[k >> 2] |= ((unsigned)(int)rintf(y[k]) & 255u) << (8 * (k & 3));
+        for (int k = 0; k < 2; ++k) {
+            unsigned w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(fmaf(f[4 * k + i], s, 12582912.f));
+            c[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400u), __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u), 0x05040100u);
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * k], y[4 * k + 1], 0, false);
-            c[k] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * k + 2], y[4 * k + 3], w, true);
+            const int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k] * s, f[4 * k + 1] * s, 0, false);
+            c[k] = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k + 2] * s, f[4 * k + 3] * s, w, true);
         }
     }
     return c;
 }
 __device__ __forceinline__ void decode8(u32x2 c, int byte, int format, float* f) {
-    if (byte == 0 || byte == 255) {
-        const float v = byte ? __builtin_nanf("") : 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = v;
-        return;
-    }
+    // 2^(byte - 127); an empty slot's factor is 0, a lost row's NaN (times any code)
+    const float s = byte == 255 ? __builtin_nanf("") : __uint_as_float((unsigned)byte << 23);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         if (format == VDA_CACHE_I8) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) f[4 * k + i] = (float)(int)(signed char)(c[k] >> (8 * i));
         } else {
+            if (byte == 0) c[k] = 0;                                // (an empty slot may hold e4m3's NaN)
             const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c[k], true);
             f[4 * k] = lo[0]; f[4 * k + 1] = lo[1]; f[4 * k + 2] = hi[0]; f[4 * k + 3] = hi[1];
         }
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = __builtin_amdgcn_ldexpf(f[k], byte - 127);
+    for (int k = 0; k < 8; ++k) f[k] = byte == 0 ? 0.f : f[k] * s;
 }
 
 struct CacheDims {
@@ -177,37 +246,60 @@ __device__ __forceinline__ void rotated4(const T* p, int e0, int half, const flo
 
 // A workgroup stores `tb` tokens (a power of two), LPH lanes of 8 channels for each (head, token), tokens fastest: the codes of a
 // head's consecutive slots are neighbours in the cache.
-enum { ROT_NONE = 0, ROT_HALVES = 1, ROT_ADJ = 2 };
+// ROT_LINE takes the other channels of the pairs from the lane `far` away, as rotary_line_kernel does; ROT_HALVES reads them.
+enum { ROT_NONE = 0, ROT_HALVES = 1, ROT_ADJ = 2, ROT_LINE = 3 };
 template <typename T, int LPH, int ROT>
 __global__ __launch_bounds__(256) void cache_write_kernel(const T* __restrict__ k, const T* __restrict__ v, CacheDims c, const long* __restrict__ slots,
-                                                          Axes ax, long rows, long ldk, long ldv, int log_tb, int format) {
+                                                          Axes ax, long rows, long ldk, long ldv, int log_tb, int format, int far) {
     extern __shared__ float2 cs[];
     __shared__ long at_row[32];
     const int tb = 1 << log_tb;
     const long r0 = (long)blockIdx.x << log_tb;
     const int nt = (int)min((long)tb, rows - r0), half = ax.half;
-    if ((int)threadIdx.x < tb) at_row[threadIdx.x] = (int)threadIdx.x < nt ? plane_row(c, slots[r0 + threadIdx.x]) : -1;
-    if (ROT != ROT_NONE)
-        for (int i = threadIdx.x; i < nt * half; i += 256) {
-            const int t = i / half;
-            cs[i] = turn(ax, r0 + t, i - t * half);
+    const int sub = threadIdx.x % LPH, e0 = sub * 8, items = c.kv_heads << log_tb;
+    // the rows of the next (head, token) are in flight while one is stored, the first ones while the angles are formed
+    Pack<T, 8> k_next = {}, v_next = {};
+    auto fetch = [&](int item) {
+        const int t = item & (tb - 1), head = item >> log_tb;
+        if (item < items && t < nt && e0 < c.hd) {
+            k_next = *reinterpret_cast<const Pack<T, 8>*>(k + (r0 + t) * ldk + (long)head * c.hd + e0);
+            v_next = *reinterpret_cast<const Pack<T, 8>*>(v + (r0 + t) * ldv + (long)head * c.hd + e0);
         }
-    __syncthreads();
-    const int sub = threadIdx.x % LPH, e0 = sub * 8;
-    for (int item = threadIdx.x / LPH; item < (c.kv_heads << log_tb); item += 256 / LPH) {
+    };
+    fetch(threadIdx.x / LPH);
+    if ((int)threadIdx.x < tb) at_row[threadIdx.x] = (int)threadIdx.x < nt ? plane_row(c, slots[r0 + threadIdx.x]) : -1;
+    if (ROT != ROT_NONE) angles(cs, ax, r0, nt);                   // (ends with a barrier)
+    else __syncthreads();
+    for (int item = threadIdx.x / LPH; item < items; item += 256 / LPH) {
         const int t = item & (tb - 1), head = item >> log_tb;
         const long base = at_row[t];
-        const bool has = base >= 0 && e0 < c.hd;
-        float fk[8] = {}, fv[8] = {};
-        if (has) {
-            const T* kr = k + (r0 + t) * ldk + (long)head * c.hd;
-            if (ROT == ROT_NONE) {
-                load_f32<T, 8>(kr + e0, fk);
-            } else {
+        float fk[8], fv[8];
+        Pack<T, 8> far_k = k_next;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { fk[i] = (float)k_next.v[i]; fv[i] = (float)v_next.v[i]; }
+        fetch(item + 256 / LPH);
+        if (ROT == ROT_HALVES || ROT == ROT_ADJ) {
+            if (t < nt && e0 < c.hd) {
+                const T* kr = k + (r0 + t) * ldk + (long)head * c.hd;
                 rotated4<T, ROT == ROT_ADJ>(kr, e0, half, cs + t * half, fk);
                 rotated4<T, ROT == ROT_ADJ>(kr, e0 + 4, half, cs + t * half, fk + 4);
             }
-            load_f32<T, 8>(v + (r0 + t) * ldv + (long)head * c.hd + e0, fv);
+        }
+        if constexpr (ROT == ROT_LINE) {
+            const bool second = e0 >= half;
+            const float2* w = cs + t * half + (e0 < 2 * half ? (second ? e0 - half : e0) : 0);
+            float y[8];
+            struct Words { int w[2 * sizeof(T)]; } words = __builtin_bit_cast(Words, far_k);
+#pragma unroll
+            for (unsigned i = 0; i < 2 * sizeof(T); ++i) words.w[i] = __shfl_xor(words.w[i], far);
+            far_k = __builtin_bit_cast(Pack<T, 8>, words);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float q = (float)far_k.v[i];
+                y[i] = fk[i] * w[i].x + (second ? q : -q) * w[i].y;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) fk[i] = e0 < 2 * half ? y[i] : fk[i];
         }
         unsigned ak = 0, av = 0;             // magnitudes as bits: they order as integers do, with NaN above infinity
 #pragma unroll
@@ -275,20 +367,20 @@ int log_tokens(long rows, int most) {
 
 template <typename T>
 int launch_rotary(const T* x, T* out, const Axes& ax, long rows, long ldx, long ldo, int heads, int hd, int pairing, hipStream_t st) {
-    const bool in_place = x == out && ldx == ldo;
-    const bool wide = sizeof(T) == 2 && pairing == VDA_PAIR_HALVES && ax.half % 8 == 0 && aligned(x, ldx, 16, 2) && aligned(out, ldo, 16, 2);
-    const int need = sizeof(T) == 2 ? (pairing == VDA_PAIR_HALVES && in_place ? 8 : 16) : 16;
-    if (!wide && (!aligned(x, ldx, need, sizeof(T)) || !aligned(out, ldo, need, sizeof(T)))) return VDA_ESHAPE;
-    const int copies = in_place ? 0 : (hd - 2 * ax.half) / (sizeof(T) == 2 ? 8 : 4);
+    constexpr int size = sizeof(T), N = 16 / size;
+    const bool in_place = x == out, adjacent = pairing == VDA_PAIR_ADJACENT, wide = aligned(x, ldx, 16, size) && aligned(out, ldo, 16, size);
+    const int far = ax.half / N;                                  // pieces between the channels of a pair
+    const bool line = wide && (adjacent || (ax.half % N == 0 && (far & (far - 1)) == 0 && far <= 32 && (hd / N) % (2 * far) == 0));
+    if (!wide && (size == 4 || adjacent || !in_place || !aligned(x, ldx, 8, size))) return VDA_ESHAPE;
     const int tb = 1 << log_tokens(rows, 16);
     const long grid = (rows + tb - 1) / tb;
     if (grid > 0x7fffffffL) return VDA_ESHAPE;
     const size_t lds = (size_t)tb * ax.half * sizeof(float2);
-#define VDA_ROT(U, ADJ) hipLaunchKernelGGL((rotary_kernel<T, U, ADJ>), dim3(grid), dim3(256), lds, st, x, out, ax, rows, ldx, ldo, heads, hd, tb, copies)
-    if (pairing == VDA_PAIR_ADJACENT) VDA_ROT(4, true);
-    else if (wide) VDA_ROT(8, false);
-    else VDA_ROT(4, false);
-#undef VDA_ROT
+    const int per_head = line ? hd / N : ax.half / 4 + (in_place ? 0 : (hd - 2 * ax.half) / (size == 2 ? 8 : 4));
+    const RotaryShape s{rows, ldx, ldo, heads, hd, tb, per_head, far, Quick(per_head * heads), Quick(per_head)};
+    if (line && adjacent) hipLaunchKernelGGL((rotary_line_kernel<T, true>), dim3(grid), dim3(256), lds, st, x, out, ax, s);
+    else if (line) hipLaunchKernelGGL((rotary_line_kernel<T, false>), dim3(grid), dim3(256), lds, st, x, out, ax, s);
+    else hipLaunchKernelGGL((rotary_pairs_kernel<T>), dim3(grid), dim3(256), lds, st, x, out, ax, s);
     return hip_rc(hipGetLastError());
 }
 
@@ -309,7 +401,7 @@ extern "C" int vda_rotary_axes(const void* x, void* out, const void* pos, const 
     if (const int rc = axes_check(pos, freq, n_t, n_h, n_w, pairing, hd)) return rc;
     if (x == out && ldx != ldo) return VDA_EINVAL;
     if (hd % 8 != 0 || hd > 256 || heads > 65536 || rows > (1L << 40) || ldx < (long)heads * hd || ldo < (long)heads * hd) return VDA_ESHAPE;
-    const Axes ax{pos, freq, n_t + n_h + n_w, n_t, n_t + n_h, pos_float};
+    const Axes ax{pos, freq, n_t + n_h + n_w, n_t, n_t + n_h, pos_float, Quick(n_t + n_h + n_w)};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (dtype == VDA_T_BF16) return launch_rotary((const bf16*)x, (bf16*)out, ax, rows, ldx, ldo, heads, hd, pairing, st);
     if (dtype == VDA_T_F16) return launch_rotary((const f16*)x, (f16*)out, ax, rows, ldx, ldo, heads, hd, pairing, st);
@@ -326,17 +418,20 @@ extern "C" int vda_cache_write(const VdaTokenCache* cache, const void* k, const 
     const int size = dtype == VDA_T_F32 ? 4 : 2;
     const long width = (long)cache->kv_heads * cache->hd;
     if (ldk < width || ldv < width || !aligned(k, ldk, 16, size) || !aligned(v, ldv, 16, size)) return VDA_ESHAPE;
-    const Axes ax{pos, freq, pos ? n_t + n_h + n_w : 0, n_t, n_t + n_h, pos_float};
+    const Axes ax{pos, freq, pos ? n_t + n_h + n_w : 0, n_t, n_t + n_h, pos_float, Quick(pos ? n_t + n_h + n_w : 1)};
     const int log_tb = log_tokens(rows, 32);
     const long grid = (rows + (1L << log_tb) - 1) >> log_tb;
     if (grid > 0x7fffffffL) return VDA_ESHAPE;
     const size_t lds = ((size_t)ax.half << log_tb) * sizeof(float2);
-    const int rot = !pos ? ROT_NONE : pairing == VDA_PAIR_HALVES ? ROT_HALVES : ROT_ADJ;
+    const int far = ax.half / 8;
+    const bool line = pos && ax.half % 8 == 0 && (far & (far - 1)) == 0 && (cache->hd / 8) % (2 * far) == 0;
+    const int rot = !pos ? ROT_NONE : pairing == VDA_PAIR_ADJACENT ? ROT_ADJ : line ? ROT_LINE : ROT_HALVES;
     const CacheDims c = dims_of(cache);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
 #define VDA_CW3(T, L, R) hipLaunchKernelGGL((cache_write_kernel<T, L, R>), dim3(grid), dim3(256), lds, st, (const T*)k, (const T*)v, c, (const long*)slots, \
-                                            ax, rows, ldk, ldv, log_tb, cache->format)
-#define VDA_CW2(T, L) do { if (rot == ROT_NONE) VDA_CW3(T, L, ROT_NONE); else if (rot == ROT_HALVES) VDA_CW3(T, L, ROT_HALVES); else VDA_CW3(T, L, ROT_ADJ); } while (0)
+                                            ax, rows, ldk, ldv, log_tb, cache->format, far)
+#define VDA_CW2(T, L) do { if (rot == ROT_NONE) VDA_CW3(T, L, ROT_NONE); else if (rot == ROT_HALVES) VDA_CW3(T, L, ROT_HALVES); \
+                           else if (rot == ROT_ADJ) VDA_CW3(T, L, ROT_ADJ); else VDA_CW3(T, L, ROT_LINE); } while (0)
 #define VDA_CW(T) do { switch (log_lanes(cache->hd)) { case 1: VDA_CW2(T, 2); break; case 2: VDA_CW2(T, 4); break; case 3: VDA_CW2(T, 8); break; \
                        default: VDA_CW2(T, 16); } } while (0)
     if (dtype == VDA_T_BF16) VDA_CW(bf16);

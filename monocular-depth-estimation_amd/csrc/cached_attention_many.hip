@@ -57,7 +57,7 @@ __device__ __forceinline__ void scaled16(u32x4 w, int e, f16x8& lo, f16x8& hi) {
     hi = f16x8{h[4][0], h[4][1], h[5][0], h[5][1], h[6][0], h[6][1], h[7][0], h[7][1]};
 }
 
-template <typename T, int HDP, int FMT, int NQ>
+template <typename T, int HDP, int FMT>
 __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void attend_many_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int groups) {
     constexpr int NP = Pieces<T>::n, KS = HDP / 16, DB = HDP / 32, CPR = HDP / 16, NC = (HDP + 63) / 64, SHIFT = FMT == VDA_CACHE_I8 ? 8 : 6;
     constexpr int PLANE = TK * HDP * 2, BUF = 2 * PLANE;
@@ -67,30 +67,20 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
     // row blocks of one (sequence, key head, split) follow each other on one XCD and share its copy of the keys
-    int id = xcd_contiguous(blockIdx.x, groups);
-    const int rb = id % j.row_blocks;
-    id /= j.row_blocks;
-    const int split = id % j.splits;
-    id /= j.splits;
-    const int kvh = id % j.kv_heads, s = id / j.kv_heads;
+    const int id = xcd_contiguous(blockIdx.x, groups);
+    const int t0 = j.by_blocks.over(id), rb = id - t0 * j.row_blocks, t1 = j.by_splits.over(t0), split = t0 - t1 * j.splits;
+    const int s = j.by_heads.over(t1), kvh = t1 - s * j.kv_heads;
     const Span sp = span_of(j, s, max_q);
     const int n_rho = sp.nq * j.group;
-    constexpr int BLOCK = 128 * NQ;
-    if (rb * BLOCK >= n_rho || split * j.chunk >= max(sp.n, 1)) return;      // the whole workgroup
-    bool live[NQ];
-    int head[NQ], limit[NQ], least = 0x7fffffff, most = 0;        // keys that a row, the wave's rows, the workgroup's rows see
-    long row[NQ];
-#pragma unroll
-    for (int b = 0; b < NQ; ++b) {
-        const int rho = rb * BLOCK + (wave * NQ + b) * 32 + r, token = rho / j.group;
-        live[b] = rho < n_rho;
-        head[b] = kvh * j.group + (rho - token * j.group);
-        row[b] = sp.q0 + (live[b] ? token : 0);
-        limit[b] = live[b] ? sp.n : 0;
-        if (j.visible && live[b]) limit[b] = max(0, min(limit[b], j.visible[row[b]]));
-        if (live[b]) least = min(least, limit[b]);
-        most = max(most, limit[b]);
-    }
+    if (rb * 128 >= n_rho || split * j.chunk >= max(sp.n, 1)) return;      // the whole workgroup
+    const int rho = rb * 128 + wave * 32 + r, token = j.by_group.over(rho), head = kvh * j.group + (rho - token * j.group);
+    const bool live = rho < n_rho;
+    const long row = sp.q0 + (live ? token : 0);
+
+    // keys that a row, the wave's rows, the workgroup's rows see
+    int limit = live ? sp.n : 0, least = live ? sp.n : 0x7fffffff, most;
+    if (j.visible && live) limit = least = max(0, min(limit, j.visible[row]));
+    most = limit;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         most = max(most, __shfl_xor(most, o));
@@ -99,25 +89,19 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
     if (lane == 0) wave_top[wave] = most;
     least = __builtin_amdgcn_readfirstlane(least);
     __syncthreads();
-    most = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
+    most = __builtin_amdgcn_readfirstlane(max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3])));
     __syncthreads();
     const int k_begin = split * j.chunk, k_end = min(k_begin + j.chunk, most);
 
     const int* table = j.page_table + (long)s * j.max_pages;
-    // the row of a plane where key `key` of this sequence lies, -1 without a page
-    auto plane_row = [&](int pi, int off) -> long {
-        const int page = table[pi];
-        return page >= 0 && page < j.pages ? ((long)page * j.kv_heads + kvh) * j.page_size + off : -1L;
-    };
-
     // the largest exponents of the part's keys and values
     int k_ref, v_ref;
     {
         int tk = 1, tv = 1;
         for (int b = (k_begin >> 4) + tid; b * 16 < k_end; b += 256) {
-            const int key = b * 16, pi = key / j.page_size;
-            const long at = plane_row(pi, key - pi * j.page_size);
-            if (at < 0) continue;
+            const int key = b * 16, pi = j.by_page.over(key), page = table[pi];
+            if (page < 0 || page >= j.pages) continue;
+            const long at = ((long)page * j.kv_heads + kvh) * j.page_size + key - pi * j.page_size;
             const u32x4 e = *reinterpret_cast<const u32x4*>(j.k_exp + at), w = *reinterpret_cast<const u32x4*>(j.v_exp + at);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -129,28 +113,27 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
         for (int o = 1; o < 64; o <<= 1) { tk = max(tk, __shfl_xor(tk, o)); tv = max(tv, __shfl_xor(tv, o)); }
         if (lane == 0) { wave_top[wave] = tk; wave_top[4 + wave] = tv; }
         __syncthreads();
-        k_ref = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
-        v_ref = max(max(wave_top[4], wave_top[5]), max(wave_top[6], wave_top[7]));
+        k_ref = __builtin_amdgcn_readfirstlane(max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3])));
+        v_ref = __builtin_amdgcn_readfirstlane(max(max(wave_top[4], wave_top[5]), max(wave_top[6], wave_top[7])));
     }
 
-    f16x8 qf[NQ][KS][NP];
-    float c_row[NQ];                                              // from products of halves to octaves
-#pragma unroll
-    for (int b = 0; b < NQ; ++b) {
+    f16x8 qf[KS][NP];
+    float c_row;                                                  // from products of halves to octaves
+    {
         float f[KS][8], amax = 0.f;
-        const T* qr = q + row[b] * j.ldq + (long)head[b] * j.hd;
+        const T* qr = q + row * j.ldq + (long)head * j.hd;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             const int e = 16 * i + 8 * h;
-            query8<T>(qr + e, live[b] && e < j.hd, f[i]);
+            query8<T>(qr + e, live && e < j.hd, f[i]);
 #pragma unroll
             for (int x = 0; x < 8; ++x) amax = fmaxf(amax, fabsf(f[i][x]));
         }
         amax = fmaxf(amax, __shfl_xor(amax, 32));
         const int shift = query_shift(amax);
 #pragma unroll
-        for (int i = 0; i < KS; ++i) query_pieces<NP>(f[i], shift, qf[b][i]);
-        c_row[b] = __builtin_amdgcn_ldexpf(j.scale_log2e, k_ref - 127 - SHIFT - shift);
+        for (int i = 0; i < KS; ++i) query_pieces<NP>(f[i], shift, qf[i]);
+        c_row = __builtin_amdgcn_ldexpf(j.scale_log2e, k_ref - 127 - SHIFT - shift);
     }
 
     // staging: wave w brings the sixteen keys 16 w .. 16 w + 15 of every tile, which lie in one page, part i of a lane being the codes
@@ -168,39 +151,49 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
         s_v[i] = PLANE + vtile<HDP>(16 * wave + s_key[i], 32 * c);
     }
     const bool do_k = HDP != 32 || lane < 32, do_v = HDP != 32 || lane >= 32;
-    int pi = (k_begin + 16 * wave) / j.page_size, off = k_begin + 16 * wave - pi * j.page_size;
-    const int step_pages = TK / j.page_size, step_off = TK - step_pages * j.page_size;
-    long at = -1;                                                 // the block's first row in the planes, -1 without a page
+    int pi = j.by_page.over(k_begin + 16 * wave), off = k_begin + 16 * wave - pi * j.page_size;
+    const int step_pages = j.by_page.over(TK), step_off = TK - step_pages * j.page_size;
+    // the page is asked for one tile ahead, from constant memory: a scalar load, which no other load has to be waited for
+    typedef const int __attribute__((address_space(4)))* constant;
+    const constant pages = (constant)table;
+    int page = pages[min(pi, j.max_pages - 1)], k_next = k_begin + 16 * wave;
     u32x4 k_code[NC], v_code[NC];
     int k_exp[NC], v_exp[NC], in_block = 0;                       // in_block: keys of the block that are there
-    auto locate = [&](int k0) {                                   // the tile at k0; advances to the next one
-        in_block = min(16, k_end - k0 - 16 * wave);
-        at = in_block > 0 ? plane_row(pi, off) : -1L;
+    auto fetch = [&]() {                                          // the next tile
+        in_block = min(16, k_end - k_next);
+        if (page < 0 || page >= j.pages) in_block = 0;
+        const long a = in_block > 0 ? ((long)page * j.kv_heads + kvh) * j.page_size + off : 0L;      // (rows 0 .. 15 exist; they are read and not used)
+        // (uniform: kept as scalar bases with 32-bit offsets, not summed into vector registers; global memory, said aloud, because a
+        // pointer that passes through here otherwise becomes a flat one, whose loads the LDS waits would wait for)
+        typedef const uint8_t __attribute__((address_space(1)))* global;
+        global kr = (global)(j.k + a * j.row_bytes), vr = (global)(j.v + a * j.row_bytes), ke = (global)(j.k_exp + a), ve = (global)(j.v_exp + a);
+        asm("" : "+s"(kr), "+s"(vr), "+s"(ke), "+s"(ve));
+        typedef const u32x4 __attribute__((address_space(1)))* global16;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const unsigned o = s_key[i] * j.row_bytes + s_col[i];
+            if (HDP == 32) {
+                k_code[i] = v_code[i] = *(global16)((do_k ? kr : vr) + o);
+            } else {
+                k_code[i] = *(global16)(kr + o);
+                v_code[i] = *(global16)(vr + o);
+            }
+            k_exp[i] = ke[(unsigned)s_key[i]];
+            v_exp[i] = ve[(unsigned)s_key[i]];
+        }
         pi += step_pages;
         off += step_off;
         if (off >= j.page_size) { off -= j.page_size; ++pi; }
-    };
-    auto fetch = [&]() {
-        const long a = at < 0 ? 0 : at;                           // (rows 0 .. 15 exist; what they hold is not used)
-        const uint8_t *kr = j.k + a * j.row_bytes, *vr = j.v + a * j.row_bytes;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int o = s_key[i] * j.row_bytes + s_col[i];
-            if (HDP == 32) {
-                k_code[i] = *reinterpret_cast<const u32x4*>((do_k ? kr : vr) + o);
-                v_code[i] = k_code[i];
-            } else {
-                k_code[i] = *reinterpret_cast<const u32x4*>(kr + o);
-                v_code[i] = *reinterpret_cast<const u32x4*>(vr + o);
-            }
-            k_exp[i] = j.k_exp[a + s_key[i]];
-            v_exp[i] = j.v_exp[a + s_key[i]];
-            if (at < 0 || s_key[i] >= in_block) k_exp[i] = 0;
-        }
+        k_next += TK;
+        page = pages[min(pi, j.max_pages - 1)];
     };
     auto store = [&](int buf) {
         char* b = smem + buf * BUF;
         bool odd = false;                                         // some key of the block is hidden or not a number
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            if (s_key[i] >= in_block) k_exp[i] = 0;
+        }
 #pragma unroll
         for (int i = 0; i < NC; ++i) odd |= k_exp[i] == 0 || k_exp[i] == 255 || v_exp[i] == 255;
         const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
@@ -234,93 +227,78 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
     };
 
     // scores are formed relative to the running maximum (0 until the row has seen a key: then it moves there whatever its sign)
-    f32x16 o[NQ][DB];
-    float m_run[NQ], l_run[NQ];                                   // l_run: of probabilities times 2^P_SHIFT
-    bool unset[NQ];
+    f32x16 o[DB];
 #pragma unroll
-    for (int b = 0; b < NQ; ++b) {
-        m_run[b] = l_run[b] = 0.f;
-        unset[b] = true;
+    for (int i = 0; i < DB; ++i)
 #pragma unroll
-        for (int i = 0; i < DB; ++i)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) o[b][i][x] = 0.f;
-    }
+        for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
+    float m_run = 0.f, l_run = 0.f;                               // l_run: of probabilities times 2^P_SHIFT
+    bool unset = true;
+    const int tq = (lane & 15) >> 2, tp = lane & 3, tcol = 2 * (16 * ((lane >> 4) & 1) + 4 * tp);
 
     if (k_begin < k_end) {
-        locate(k_begin);
         fetch();
-        locate(k_begin + TK);
         store(0);
     }
     __syncthreads();
-    const int tq = (lane & 15) >> 2, tp = lane & 3, tcol = 2 * (16 * ((lane >> 4) & 1) + 4 * tp);
     int cur = 0;
     for (int k0 = k_begin; k0 < k_end; k0 += TK, cur ^= 1) {
         fetch();                                                  // of the tile after this one, or of nothing
-        locate(k0 + 2 * TK);
         const char* kb = smem + cur * BUF;
         const char* vb = kb + PLANE;
         const unsigned long hidden = __builtin_amdgcn_ballot_w64(hide[cur][lane] != 0);
         // 32 keys at a time: half the registers for scores and probabilities
 #pragma unroll
         for (int kh = 0; kh < 2; ++kh) {
-            f32x16 sc[NQ];
+            f32x16 sc;
 #pragma unroll
-            for (int b = 0; b < NQ; ++b)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) sc[b][x] = 0.f;
+            for (int x = 0; x < 16; ++x) sc[x] = 0.f;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
                 const f16x8 kf = *reinterpret_cast<const f16x8*>(kb + ktile<HDP>(32 * kh + r, 2 * i + h));
 #pragma unroll
-                for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-                    for (int b = 0; b < NQ; ++b) sc[b] = mfma32(kf, qf[b][i][p], sc[b]);
+                for (int p = NP - 1; p >= 0; --p) sc = mfma32(kf, qf[i][p], sc);
             }
             const unsigned gone = (unsigned)(kh ? hidden >> 32 : hidden);
-            f16x8 pf[NQ][2][NP];
+            const float base = (float)P_SHIFT - m_run;
 #pragma unroll
-            for (int b = 0; b < NQ; ++b) {
-                const float base = (float)P_SHIFT - m_run[b];
-#pragma unroll
-                for (int x = 0; x < 16; ++x) sc[b][x] = fmaf(sc[b][x], c_row[b], base);
-                if (gone != 0 || k0 + 32 * kh + 32 > least) {
-                    const unsigned mine = gone >> (4 * h);
-                    const int left = limit[b] - (k0 + 32 * kh + 4 * h);
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const int in32 = (x & 3) + 8 * (x >> 2);  // + 4 h
-                        if ((mine >> in32 & 1) || in32 >= left) sc[b][x] = -INFINITY;
-                    }
-                }
-                float mx = sc[b][0];
-#pragma unroll
-                for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sc[b][x]);
-                if (__builtin_amdgcn_ballot_w64(mx > DEFER + P_SHIFT || (unset[b] && mx > -INFINITY)) != 0) {
-                    mx = fmaxf(mx, __shfl_xor(mx, 32)) - P_SHIFT;
-                    const float delta = !unset[b] ? fmaxf(mx, 0.f) : mx == -INFINITY ? 0.f : mx, alpha = unset[b] ? 1.f : __builtin_amdgcn_exp2f(-delta);
-                    unset[b] = unset[b] && mx == -INFINITY;
-                    m_run[b] += delta;
-                    l_run[b] *= alpha;
-#pragma unroll
-                    for (int i = 0; i < DB; ++i)
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) o[b][i][x] *= alpha;
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) sc[b][x] -= delta;
-                }
-                float sum[2] = {0.f, 0.f};
+            for (int x = 0; x < 16; ++x) sc[x] = fmaf(sc[x], c_row, base);
+            if (gone != 0 || k0 + 32 * kh + 32 > least) {
+                const unsigned mine = gone >> (4 * h);
+                const int left = limit - (k0 + 32 * kh + 4 * h);
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const float p = __builtin_amdgcn_exp2f(sc[b][x]);
-                    sum[x & 1] += p;
-                    const f16 hi = (f16)p;
-                    pf[b][x >> 3][0][x & 7] = hi;
-                    if (NP == 2) pf[b][x >> 3][NP - 1][x & 7] = (f16)(p - (float)hi);
+                    const int in32 = (x & 3) + 8 * (x >> 2);      // + 4 h
+                    if ((mine >> in32 & 1) || in32 >= left) sc[x] = -INFINITY;
                 }
-                l_run[b] += sum[0] + sum[1];
             }
+            float mx = sc[0];
+#pragma unroll
+            for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sc[x]);
+            if (__builtin_amdgcn_ballot_w64(mx > DEFER + P_SHIFT || (unset && mx > -INFINITY)) != 0) {
+                mx = fmaxf(mx, __shfl_xor(mx, 32)) - P_SHIFT;
+                const float delta = !unset ? fmaxf(mx, 0.f) : mx == -INFINITY ? 0.f : mx, alpha = unset ? 1.f : __builtin_amdgcn_exp2f(-delta);
+                unset = unset && mx == -INFINITY;
+                m_run += delta;
+                l_run *= alpha;
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) o[i][x] *= alpha;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) sc[x] -= delta;
+            }
+            float sum[2] = {0.f, 0.f};
+            f16x8 pf[2][NP];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const float p = __builtin_amdgcn_exp2f(sc[x]);
+                sum[x & 1] += p;
+                const f16 hi = (f16)p;
+                pf[x >> 3][0][x & 7] = hi;
+                if (NP == 2) pf[x >> 3][NP - 1][x & 7] = (f16)(p - (float)hi);
+            }
+            l_run += sum[0] + sum[1];
 #pragma unroll
             for (int i = 0; i < DB; ++i)
 #pragma unroll
@@ -329,55 +307,50 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
                     const f16x4 lo = read_tr<f16>(vb + vtile<HDP>(key, 64 * i + tcol)), hi = read_tr<f16>(vb + vtile<HDP>(key + 8, 64 * i + tcol));
                     const f16x8 vf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
-                    for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-                        for (int b = 0; b < NQ; ++b) o[b][i] = mfma32(vf, pf[b][x][p], o[b][i]);
+                    for (int p2 = NP - 1; p2 >= 0; --p2) o[i] = mfma32(vf, pf[x][p2], o[i]);
                 }
         }
         store(cur ^ 1);
         __syncthreads();
     }
 
-    // lane (r, h) holds channels 32 i + 8 g + 4 h + 0..3 of query r in o[.][i][4 g + 0..3]
-    float* part = j.part + ((((long)s * j.row_blocks + rb) * j.kv_heads + kvh) * j.splits + split) * (BLOCK * (HDP + 2));
-#pragma unroll
-    for (int b = 0; b < NQ; ++b) {
-        const float l = l_run[b] + __shfl_xor(l_run[b], 32);
-        if (!live[b]) continue;
-        if (j.splits > 1) {
-            const int in_block = (wave * NQ + b) * 32 + r;
-            float* d = part + in_block * HDP + 4 * h;
-#pragma unroll
-            for (int i = 0; i < DB; ++i)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    f32x4 v;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) v[x] = __builtin_amdgcn_ldexpf(o[b][i][4 * g + x], v_ref - 127 - SHIFT);
-                    *reinterpret_cast<f32x4*>(d + 32 * i + 8 * g) = v;
-                }
-            if (h == 0) { part[BLOCK * HDP + in_block] = unset[b] ? LOWEST : m_run[b]; part[BLOCK * HDP + BLOCK + in_block] = l; }
-            continue;
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        T* orow = out + row[b] * j.ldo + (long)head[b] * j.hd + 4 * h;
+    // lane (r, h) holds channels 32 i + 8 g + 4 h + 0..3 of query r in o[i][4 g + 0..3]
+    const float l = l_run + __shfl_xor(l_run, 32);
+    if (!live) return;
+    if (j.splits > 1) {
+        float* part = j.part + ((((long)s * j.row_blocks + rb) * j.kv_heads + kvh) * j.splits + split) * (128 * (HDP + 2));
+        const int in_wg = wave * 32 + r;
+        float* d = part + in_wg * HDP + 4 * h;
 #pragma unroll
         for (int i = 0; i < DB; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                if (32 * i + 8 * g >= j.hd) continue;
-                typename Vec<T>::v4 v;
+                f32x4 v;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) v[x] = (T)(__builtin_amdgcn_ldexpf(o[b][i][4 * g + x], v_ref - 127 - SHIFT) * inv);
-                *reinterpret_cast<typename Vec<T>::v4*>(orow + 32 * i + 8 * g) = v;
+                for (int x = 0; x < 4; ++x) v[x] = __builtin_amdgcn_ldexpf(o[i][4 * g + x], v_ref - 127 - SHIFT);
+                *reinterpret_cast<f32x4*>(d + 32 * i + 8 * g) = v;
             }
+        if (h == 0) { part[128 * HDP + in_wg] = unset ? LOWEST : m_run; part[128 * HDP + 128 + in_wg] = l; }
+        return;
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* orow = out + row * j.ldo + (long)head * j.hd + 4 * h;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (32 * i + 8 * g >= j.hd) continue;
+            typename Vec<T>::v4 v;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = (T)(__builtin_amdgcn_ldexpf(o[i][4 * g + x], v_ref - 127 - SHIFT) * inv);
+            *reinterpret_cast<typename Vec<T>::v4*>(orow + 32 * i + 8 * g) = v;
+        }
 }
 
 template <typename T>
 int many(const AttendJob& j, const T* q, T* out, int format, int max_q, hipStream_t st) {
     const int groups = j.seqs * j.kv_heads * j.row_blocks * j.splits;
-#define VDA_M2(H, F) hipLaunchKernelGGL((attend_many_kernel<T, H, F, 1>), dim3(groups), dim3(256), 0, st, q, out, j, max_q, groups)
+#define VDA_M2(H, F) hipLaunchKernelGGL((attend_many_kernel<T, H, F>), dim3(groups), dim3(256), 0, st, q, out, j, max_q, groups)
 #define VDA_M(H) do { if (format == VDA_CACHE_I8) VDA_M2(H, VDA_CACHE_I8); else VDA_M2(H, VDA_CACHE_E4M3); } while (0)
     if (j.hd <= 32) VDA_M(32);
     else if (j.hd <= 64) VDA_M(64);

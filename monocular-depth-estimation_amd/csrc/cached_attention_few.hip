@@ -56,48 +56,70 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP, FMT, W>()
 
     // this lane's part of a V tile: it copies 16 bytes of HDP / 32 keys
     char* vt = smem + wave * (32 * HDP);
-    int v_key[CB], v_col[CB], v_lds[CB];
+    int v_key[CB], v_lds[CB];
+    unsigned v_off[CB], k_off[C64 + TAIL32];                        // bytes from a block's first row
 #pragma unroll
     for (int i = 0; i < CB; ++i) {
         const int idx = i * 64 + lane;
         v_key[i] = idx / (HDP / 16);
         const int col = (idx % (HDP / 16)) * 16;
-        v_col[i] = min(col, j.row_bytes - 16);
+        v_off[i] = (v_key[i] & 15) * j.row_bytes + min(col, j.row_bytes - 16);
         v_lds[i] = vtile<HDP>(v_key[i], col);
     }
-    const int k_off8 = min(64 * C64 + 8 * g, j.row_bytes - 8);
+#pragma unroll
+    for (int i = 0; i < C64; ++i) k_off[i] = c16 * j.row_bytes + min(64 * i + 16 * g, j.row_bytes - 16);
+    if (TAIL32) k_off[C64] = c16 * j.row_bytes + min(64 * C64 + 8 * g, j.row_bytes - 8);
 
-    // the pages of a step's two blocks of 16 keys (a page holds a multiple of 16 slots); a block without one reads as empty slots
-    const int* table = j.page_table + (long)s * j.max_pages;
-    int pi = j.by_page.over(k_begin), off = k_begin - pi * j.page_size;
-    auto block_row = [&]() -> long {
-        long r = -1;
-        if (pi < j.max_pages) {
-            const int page = table[pi];
-            if (page >= 0 && page < j.pages) r = ((long)page * j.kv_heads + kvh) * j.page_size + off;
-        }
-        off += 16;
-        if (off >= j.page_size) { off = 0; ++pi; }
-        return r;
+    // A step has two blocks of 16 keys, each in one page (a page holds a multiple of 16 slots); a block without one reads as empty
+    // slots.  Pages are asked for one step ahead, from constant memory: scalar loads, for which no other load has to be waited.
+    typedef const int __attribute__((address_space(4)))* constant;
+    typedef const uint8_t __attribute__((address_space(1)))* global;
+    typedef const unsigned __attribute__((address_space(1)))* global4;
+    typedef const u32x2 __attribute__((address_space(1)))* global8;
+    typedef const u32x4 __attribute__((address_space(1)))* global16;
+    const constant table = (constant)(j.page_table + (long)s * j.max_pages);
+    int pi[2], off[2], page[2];
+    pi[0] = j.by_page.over(k_begin);
+    off[0] = k_begin - pi[0] * j.page_size;
+    auto next_block = [&](int from, int to) {
+        pi[to] = pi[from];
+        off[to] = off[from] + 16;
+        if (off[to] >= j.page_size) { off[to] = 0; ++pi[to]; }
     };
+    auto ask = [&]() {
+        next_block(0, 1);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int x = table[min(pi[b], j.max_pages - 1)];
+            page[b] = pi[b] < j.max_pages ? x : -1;
+        }
+    };
+    ask();
     auto fetch = [&](Step<HDP>& st) {
         long r[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            r[b] = block_row();
-            const bool any = r[b] >= 0;
-            if (!any) r[b] = 0;                                     // slot 0 exists: its bytes are read and not used
-            const uint8_t* kr = j.k + (r[b] + c16) * j.row_bytes;
+            const bool any = page[b] >= 0 && page[b] < j.pages;
+            r[b] = any ? ((long)page[b] * j.kv_heads + kvh) * j.page_size + off[b] : 0L;      // rows 0 .. 15 exist: they are read and not used
+            // (global memory, said aloud, with scalar bases and 32-bit offsets of the lanes)
+            global kr = (global)(j.k + r[b] * j.row_bytes), ke = (global)(j.k_exp + r[b]), ve = (global)(j.v_exp + r[b]);
+            asm("" : "+s"(kr), "+s"(ke), "+s"(ve));
 #pragma unroll
-            for (int i = 0; i < C64; ++i) st.k[b][i] = *reinterpret_cast<const u32x4*>(kr + min(64 * i + 16 * g, j.row_bytes - 16));
-            if (TAIL32) st.k8[b] = *reinterpret_cast<const u32x2*>(kr + k_off8);
-            st.ek[b] = *reinterpret_cast<const unsigned*>(j.k_exp + r[b] + 4 * g);
-            st.ev[b] = *reinterpret_cast<const unsigned*>(j.v_exp + r[b] + 4 * g);
+            for (int i = 0; i < C64; ++i) st.k[b][i] = *(global16)(kr + k_off[i]);
+            if (TAIL32) st.k8[b] = *(global8)(kr + k_off[C64]);
+            st.ek[b] = *(global4)(ke + 4u * g);
+            st.ev[b] = *(global4)(ve + 4u * g);
             if (!any) st.ek[b] = 0u;
         }
+        global vr[2] = {(global)(j.v + r[0] * j.row_bytes), (global)(j.v + r[1] * j.row_bytes)};
+        asm("" : "+s"(vr[0]), "+s"(vr[1]));
 #pragma unroll
-        for (int i = 0; i < CB; ++i)
-            st.v[i] = *reinterpret_cast<const u32x4*>(j.v + ((v_key[i] < 16 ? r[0] : r[1]) + (v_key[i] & 15)) * j.row_bytes + v_col[i]);
+        for (int i = 0; i < CB; ++i) {
+            if (HDP % 64 == 0) st.v[i] = *(global16)(vr[2 * i / CB] + v_off[i]);       // (a block's keys fill whole chunks of 64 lanes)
+            else st.v[i] = *(global16)((v_key[i] < 16 ? vr[0] : vr[1]) + v_off[i]);
+        }
+        next_block(1, 0);
+        ask();
     };
     // the first keys are asked for before it is known whether the sequence has them (the planes hold them in any case): the loads
     // of lengths, query rows and keys are in flight together

@@ -389,8 +389,8 @@ typedef struct VdaTokenCache {
 } VdaTokenCache;
 
 /* vda_cache_write: rows k [rows][ldk] and v [rows][ldv] (dtype BF16, F16 or F32, kv_heads * hd values each) go to the slots
- *   slots[r] = page * page_size + place (int64; a row whose slot is negative or beyond the cache is skipped; the others are
- *   distinct).  pos != NULL: the keys are turned first, as by vda_rotary_axes with heads of hd channels, in fp32 without a
+ *   slots[r] = page * page_size + place (int64; a row whose slot is negative or beyond the cache is skipped; a slot named twice in
+ *   one call holds neither row).  pos != NULL: the keys are turned first, as by vda_rotary_axes with heads of hd channels, in fp32 without a
  *   rounding in between.  16-byte aligned rows.
  * vda_cache_read: the values of the slots, rounded to dtype, into rows k and v; rows without a slot stay as they were, empty
  *   slots read as 0. */
@@ -400,12 +400,13 @@ int vda_cache_read(const VdaTokenCache* cache, const int64_t* slots, void* k, vo
 
 /* vda_cached_attention: softmax(scale * q K^T) V over the cache, for `seqs` sequences at once.  Sequence s has the query rows
  *   q_start[s] .. q_start[s+1]-1 of q (int32 [seqs + 1], cut to 0 .. rows; at most max_q of them are computed) and the keys
- *   0 .. kv_len[s]-1, key i in page page_table[s][i / page_size] (int32 [seqs][max_pages]) at place i % page_size.  Row r sees
+ *   0 .. kv_len[s]-1 (cut to max_pages * page_size, which is 2^30 at most), key i in page page_table[s][i / page_size] (int32
+ *   [seqs][max_pages]) at place i % page_size.  Row r sees
  *   the first visible[r] of its sequence's keys (int32 [rows]; NULL: all): a causal mask, by token or by frame.  Keys
  *   in empty slots and in pages outside 0 .. pages-1 (evicted ones: -1) are not seen by any row.  A row that sees no key is 0.  What
  *   is not seen has no effect, NaN included.  Query heads h * G .. h * G + G-1 use key head h, G = heads / kv_heads.
  *   q, out: dtype BF16, F16 or F32, rows of ldq and ldo elements, 16-byte aligned; rows of no sequence are left as they were.
- *   Scores, softmax and sums are fp32.  16-bit types: products of IEEE halves, the cached values exactly and the probabilities
+ *   Scores, softmax and sums are fp32 (keys beyond 1e30 overflow them).  16-bit types: products of IEEE halves, the cached values exactly and the probabilities
  *   rounded to 11 bits; F32: q and the probabilities in two pieces (22 bits).
  *   work: vda_cached_attention_work bytes of scratch, 16-byte aligned, of no meaning between calls; calls that may run at the
  *   same time need one each.  Results are the same bits from run to run. */

@@ -9,27 +9,29 @@ struct Plan {
     long work;
 };
 
-// Up to 32 rows per key head, or few rows of work in all (blocks of 16 rows times keys): the kernel whose waves hold 16 rows each and read the cache straight into registers.  It wants
-// enough waves in flight to draw the full memory bandwidth, a few thousand: where the (sequence, key head, row block) items alone
-// are fewer, four waves share an item and the key axis is split over workgroups, down to 128 keys for each wave.
+// Up to 32 rows per key head, or few rows of work in all (blocks of 16 rows times keys, fewer for wide heads): the kernel whose waves
+// hold 16 rows each and read the cache straight into registers.  It wants enough waves in flight to draw the full memory bandwidth:
+// where there are fewer than 4096 (sequence, key head, row block) items, eight waves share an item, and beyond 2048 keys the key
+// axis is split over workgroups too, down to 64 keys for each wave.
 // More rows: the kernel whose workgroups of 128 rows share decoded tiles; the key axis is split, down to 512 keys, until the
 // workgroups that a CU holds at once (three, two for wide heads) are there.
-// Measured, 8 heads of 64, us of this kernel / the other: 32 rows over 16384 keys 31 / 30, 64 rows 38 / 30; 384 rows over 2048 keys
-// 17 / 24; 8 sequences of 64 rows over 2048 keys 17 / 25, of 192 rows 34 / 36, of 384 rows 60 / 43.
-constexpr int FEW_ROWS = 32, FEW_KEYS = 4096, FEW_WORK = 3 << 18;
+// Measured, us of the first kernel / the second, 8 heads of 64 in IEEE half: 32 rows over 8192 keys 20 / 25, 96 rows 27 / 26; 384 rows
+// over 2048 keys 16 / 23; 8 sequences over 2048 keys, 96 rows 23 / 26, 256 rows 40 / 38; 64 sequences over 512 keys, 32 rows
+// 18 / 22, 64 rows 30 / 23.  Heads of 128: 8 sequences over 2048 keys, 64 rows 21 / 32, 96 rows 37 / 34; over 512 keys, 384 rows 46 / 25.
+constexpr int FEW_ROWS = 32, FEW_KEYS = 4096;
 constexpr int ONE_FEW = 2048, MIN_FEW = 512, MIN_MANY = 512;
 int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int heads, Plan* p) {
     if (const int rc = cache_check(c)) return rc;
     if (seqs <= 0 || max_pages <= 0 || max_q <= 0 || heads <= 0) return VDA_EINVAL;
-    if (heads % c->kv_heads != 0 || (long)max_pages * c->page_size > 0x7fffffffL) return VDA_ESHAPE;
+    if (heads % c->kv_heads != 0 || (long)max_pages * c->page_size > 0x40000000L) return VDA_ESHAPE;
     const long rows = (long)max_q * (heads / c->kv_heads), keys = (long)max_pages * c->page_size;
     const long few_items = (rows + 15) / 16 * seqs * c->kv_heads;
-    const bool few = rows <= FEW_ROWS || (keys <= FEW_KEYS && few_items <= FEW_WORK / keys);
+    const bool few = rows <= FEW_ROWS || (keys <= FEW_KEYS && few_items <= ((c->hd <= 64 ? 3L : 2L) << 18) / keys);
     p->block_rows = few ? 16 : 128;
     p->hd_pad = (c->hd + 31) & ~31;
     const long blocks = (rows + p->block_rows - 1) / p->block_rows, items = blocks * seqs * c->kv_heads;
-    if (rows > 0x7fffffffL || items > 0x3fffffffL) return VDA_ESHAPE;
-    long chunk = keys;                                            // keys of a part: 32 for each of eight waves, or more
+    if (rows > 0x3fffffffL || items > 0x3fffffffL) return VDA_ESHAPE;
+    long chunk = keys;                                            // keys of a part, a multiple of 32 for each of eight waves
     if (few) {
         p->waves = items >= 4096 || keys <= 64 ? 1 : 8;
         if (p->waves == 8 && keys > ONE_FEW) {
@@ -44,7 +46,6 @@ int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int head
         chunk = chunk < MIN_MANY ? MIN_MANY : chunk;
     }
     chunk = (chunk + 255) & ~255L;
-    if (chunk > 0x40000000L) return VDA_ESHAPE;
     const long splits = (keys + chunk - 1) / chunk;
     p->chunk = (int)chunk;
     p->splits = (int)splits;

@@ -15,7 +15,7 @@ static inline int cache_check(const VdaTokenCache* c) {
 }
 
 // n / d for 0 <= n < 2^31 and a divisor known when the call is made: one high product and a shift.  With l = ceil(log2 d) and
-// m = ceil(2^(31 + l) / d) the product n m / 2^(31 + l) exceeds n / d by less than n / 2^31 < 1 of 1 / d, which reaches no next integer.
+// m = ceil(2^(31 + l) / d) < 2^32, n m / 2^(31 + l) exceeds n / d by less than n / 2^(31 + l) < 2^-l <= 1 / d: the same integer part.
 struct Quick {
     unsigned d, m;
     int s;

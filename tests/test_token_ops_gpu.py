@@ -482,3 +482,177 @@ def test_gated_norm_is_the_frameworks_layernorm_on_a_plain_stream():
     hip.layernorm(x, a, w, b, 50, 1024, 1e-6)
     hip.gated_norm(x, None, None, y, rows=50, C=1024, pre_w=w, pre_b=b, eps=1e-6)
     within(y, a.double().cpu(), 2 * NORM_ERROR * (x.abs().double().cpu().amax() * w.abs().double().cpu().amax() + 4))
+
+
+# ---- calls at the ends of what is allowed ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("q_len", [1, 40])
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_attention_with_a_negative_and_a_zero_scale(q_len, scale):
+    """A negative scale prefers the keys that point away; 0 weighs all that are seen alike, and still nothing else."""
+    table_pages = 1 if q_len == 1 else 300                  # (a long table of absent pages: the kernel for many rows)
+    m = Memory([100, 33], 2, 64, 16, "i8", 101)
+    m.table = torch.nn.functional.pad(m.table, (0, table_pages), value=-1)
+    visible = torch.tensor([90] * q_len + [0] * q_len, dtype=torch.int32)
+    out = m.check(queries(2 * q_len, 4, 64, torch.float16, 102), [0, q_len, 2 * q_len], 4, scale=scale, visible=visible)[0]
+    assert bool((out[q_len:] == 0).all())
+
+
+@pytest.mark.parametrize("q_len,heads,hd", [(1, 8, 128), (64, 8, 128), (40, 16, 96)])
+def test_cache_rows_behind_4_gib(q_len, heads, hd):
+    """Planes of more than 2^32 bytes: the pages in use are the last ones and the first."""
+    kv_heads, page = 8, 64
+    pages = (1 << 32) // (page * kv_heads * hip.cache_row_bytes(hd)) + 300
+    planes = [torch.empty((pages, kv_heads, page, hip.cache_row_bytes(hd)), dtype=torch.uint8, device=DEV) for _ in range(2)]
+    planes += [torch.zeros((pages, kv_heads, page), dtype=torch.uint8, device=DEV) for _ in range(2)]
+    used = [pages - 1, 0, pages - 2, pages - 7, 1]
+    n = 4 * page + 9
+    i = torch.arange(n)
+    slots = (torch.tensor(used)[i // page] * page + i % page).to(DEV)
+    g = gen(111)
+    k, v = (torch.randn((n, kv_heads, hd), generator=g).to(DEV) for _ in range(2))
+    kw = dict(kv_heads=kv_heads, hd=hd, page_size=page, fmt=hip.CACHE_I8)
+    hip.cache_write(k, v, *planes, slots, rows=n, **kw)
+    k2, v2 = torch.empty_like(k), torch.empty_like(v)
+    hip.cache_read(*planes, slots, k2, v2, rows=n, **kw)
+    for x, y in ((k, k2), (v, v2)):
+        e = R.exponents(x.cpu(), "i8")
+        assert torch.equal(y.cpu().double(), R.codes(x.cpu(), e, "i8") * torch.exp2(e.double() - 127)[..., None])
+    q = queries(q_len, heads, hd, torch.float16, 112)
+    out = torch.empty_like(q)
+    table = torch.full((1, 5 if q_len == 1 else 500), -1, dtype=torch.int32)
+    table[0, :5] = torch.tensor(used)
+    start, length = torch.tensor([0, q_len], dtype=torch.int32), torch.tensor([n], dtype=torch.int32)
+    hip.cached_attention(q, out, *planes, table.to(DEV), length.to(DEV), start.to(DEV), heads=heads, max_q=q_len, scale=hd ** -0.5, **kw)
+    small = [p[used].contiguous() for p in planes]           # the same rows in a small cache, for the reference
+    table[0, :5] = torch.arange(5)
+    want, tol = R.attend(q, *small, table, length, start, None, heads, kv_heads, hd, page, "i8", hd ** -0.5)
+    within(out, want, tol)
+
+
+@pytest.mark.parametrize("q_len,kv", [(1, 6000), (200, 6000)])
+def test_attention_graphs_on_two_streams_with_workspaces_of_their_own(q_len, kv):
+    """Two captured calls replayed side by side, with eager calls on a third stream between, give what one call alone gives."""
+    m = Memory([kv], 2, 64, 64, "e4m3", 121)
+    table, kv_len, start = m.table.to(DEV), m.kv_len.to(DEV), torch.tensor([0, q_len], dtype=torch.int32, device=DEV)
+    shape = dict(heads=4, kv_heads=2, hd=64, page_size=64, fmt=hip.CACHE_E4M3, max_q=q_len)
+    n = hip.cached_attention_work(m.planes[0], seqs=1, max_pages=table.shape[1], **shape)
+    assert n > 0
+    qs = [queries(q_len, 4, 64, torch.bfloat16, 122 + i) for i in range(3)]
+    want = [torch.empty_like(q) for q in qs]
+    for q, w in zip(qs, want):
+        hip.cached_attention(q, w, *m.planes, table, kv_len, start, scale=0.125, **shape)
+    torch.cuda.synchronize()
+    outs, graphs, streams = [], [], [torch.cuda.Stream() for _ in range(3)]
+    works = [torch.empty(n, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    for q, work in zip(qs, works):
+        out, graph = torch.empty_like(q), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            hip.cached_attention(q, out, *m.planes, table, kv_len, start, scale=0.125, work=work, **shape)
+        outs.append(out)
+        graphs.append(graph)
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            third = torch.empty_like(qs[2])
+            hip.cached_attention(qs[2], third, *m.planes, table, kv_len, start, scale=0.125, **shape)
+        torch.cuda.synchronize()
+        for got, w in zip(outs + [third], want):
+            assert torch.equal(got, w)
+
+
+# ---- the operators together ----------------------------------------------------------------------------------------------------------
+def product_check(got, a, w):
+    """A product of 16-bit operands with fp32 sums, rounded to got's type."""
+    a, w = a.double().cpu(), w.double().cpu()
+    want, size = a @ w.t(), a.abs() @ w.abs().t()
+    e = (a.shape[1] + 8) * 2.0 ** -24 * size
+    within(got, want, e + R.half_step(got.dtype) * (want.abs() + e), "product")
+
+
+@pytest.mark.parametrize("dt,fmt,tokens,table_pages,pairing", [(torch.bfloat16, "i8", 20, 3, "halves"), (torch.float16, "e4m3", 33, 200, "adjacent"), (torch.float16, "i8", 1, 3, "halves")])
+def test_a_block_over_a_memory_of_frames(dt, fmt, tokens, table_pages, pairing):
+    """Two streams pass frame after frame through norm, projections, rotation, the cache, attention over the last three frames, the
+    output projection and the norms around it, with the oldest page given to the new frame; every step is held to its
+    definition on what the step before it left.  The last frame again on a stream of its own and as a captured graph: the same bits."""
+    streams, C, heads, kv_heads, hd, page, held = 2, 256, 4, 2, 64, 48, 3
+    rows, qw, kw_ = streams * tokens, heads * hd, kv_heads * hd
+    g = gen(131)
+    r = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    w_in, w_out = (r(qw + 2 * kw_, C) / 16).to(dt).to(DEV), (r(C, qw) / 16).to(dt).to(DEV)
+    freq = (torch.rand(hd // 2, generator=g, dtype=torch.float64)).to(DEV)
+    vec = {n: t.to(DEV) for n, t in dict(post_w=1 + 0.1 * r(C), gate=r(streams, C), pre_w=1 + 0.1 * r(C), mod_scale=0.2 * r(streams, C), mod_shift=0.1 * r(streams, C)).items()}
+    before = dict(rows=rows, C=C, pre=hip.NORM_RMS, pre_w=vec["pre_w"], mod_scale=vec["mod_scale"], mod_shift=vec["mod_shift"], rows_per_group=tokens)
+    after = dict(rows=rows, C=C, post=hip.NORM_RMS, post_w=vec["post_w"], gate=vec["gate"], pre=hip.NORM_LAYER, rows_per_group=tokens)
+    planes = new_cache(streams * held, kv_heads, page, hd)
+    shape = dict(kv_heads=kv_heads, hd=hd, page_size=page, fmt=FMT[fmt])
+    turn = dict(sections=(8, 12, 12), pairing=PAIR[pairing])
+    table = torch.full((streams, table_pages), -1, dtype=torch.int32, device=DEV)
+    kv_len, start = torch.zeros(streams, dtype=torch.int32, device=DEV), torch.arange(streams + 1, dtype=torch.int32, device=DEV) * tokens
+    slots, pos, x = torch.empty(rows, dtype=torch.int64, device=DEV), torch.empty((rows, 3), dtype=torch.int32, device=DEV), torch.empty((rows, C), device=DEV)
+    n = hip.cached_attention_work(planes[0], seqs=streams, max_pages=table_pages, max_q=tokens, heads=heads, **shape)
+    work = torch.empty(max(n, 16), dtype=torch.uint8, device=DEV)
+
+    def step():
+        y, packed, att, b = (torch.empty((rows, w), dtype=dt, device=DEV) for w in (C, qw + 2 * kw_, qw, C))
+        x_out, z = torch.empty_like(x), torch.empty((rows, C), dtype=dt, device=DEV)
+        hip.gated_norm(x, None, None, y, **before)
+        hip.gemm(y, w_in, packed, M=rows, N=qw + 2 * kw_, K=C, lda=C, ldc=qw + 2 * kw_)
+        flat = packed.clone()
+        q, k, v = packed[:, :qw], packed[:, qw:qw + kw_], packed[:, qw + kw_:]
+        hip.rotary_axes(q, q, pos, freq, rows=rows, heads=heads, hd=hd, **turn)
+        hip.cache_write(k, v, *planes, slots, rows=rows, pos=pos, freq=freq, **turn, **shape)
+        hip.cached_attention(q, att, *planes, table, kv_len, start, heads=heads, max_q=tokens, scale=hd ** -0.5, work=work, **shape)
+        hip.gemm(att, w_out, b, M=rows, N=C, K=qw, lda=qw, ldc=C)
+        hip.gated_norm(x, b, x_out, z, **after)
+        return y, flat, packed, att, b, x_out, z
+
+    for f in range(5):
+        # a stream's pages in the order of their frames; place f % held is the newest frame's, the oldest one's before
+        at = [s * held + (f - i) % held for s in range(streams) for i in reversed(range(min(f + 1, held)))]
+        table[:, :min(f + 1, held)] = torch.tensor(at, dtype=torch.int32).reshape(streams, -1).to(DEV)
+        full = min(f, held - 1)                                              # older frames; their unused places are empty slots
+        kv_len.fill_(full * page + tokens)
+        t = torch.arange(tokens)
+        slots.copy_(torch.cat([(s * held + f % held) * page + t for s in range(streams)]))
+        pos.copy_(torch.stack([torch.full((tokens,), 30 * f), t // 7, t % 7], 1).repeat(streams, 1))
+        x.copy_(r(rows, C))
+        y, flat, packed, att, b, x_out, z = step()
+        rounding = lambda want, e: e + R.half_step(dt) * (want.abs() + e)  # noqa: E731
+        _, want, _, size = R.gated_norm(x, None, "none", None, None, None, 1.0, "rms", vec["pre_w"], None, vec["mod_scale"], vec["mod_shift"], tokens, 1e-6)
+        within(y, want, rounding(want, NORM_ERROR * size), "first norm")
+        product_check(flat, y, w_in)
+        rotary_check(packed[:, :qw].reshape(rows, heads, hd), flat[:, :qw].reshape(rows, heads, hd), pos, freq, turn["sections"], pairing)
+        assert torch.equal(packed[:, qw:], flat[:, qw:])
+        p, o = slots // page, slots % page
+        want, size = R.rotate(flat[:, qw:qw + kw_].reshape(rows, kv_heads, hd), pos, freq, turn["sections"], pairing)
+        scale = torch.exp2(planes[2][p, :, o].cpu().double() - 127)[..., None]
+        code_step = torch.ones_like(want) if fmt == "i8" else torch.exp2(torch.floor(torch.log2((want / scale).abs().clamp_min(2.0 ** -6))) - 3)
+        within(R.decode(planes[0][p, :, o][..., :hd], planes[2][p, :, o], fmt), want, code_step * scale / 2 * (1 + 1e-5) + R.ROTATION * size, "keys")
+        want, tol = R.attend(packed[:, :qw].reshape(rows, heads, hd), *planes, table.cpu(), kv_len, start, None, heads, kv_heads, hd, page, fmt, hd ** -0.5)
+        within(att.reshape(rows, heads, hd), want, tol, "attention")
+        product_check(b, att, w_out)
+        want_x, want, size_x, size = R.gated_norm(x, b, "rms", vec["post_w"], None, vec["gate"], 1.0, "layer", None, None, None, None, tokens, 1e-6)
+        within(x_out, want_x, NORM_ERROR * size_x, "stream")
+        within(z, want, rounding(want, NORM_ERROR * size), "last norm")
+
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        again = step()
+    torch.cuda.synchronize()
+    assert torch.equal(again[-1], z) and torch.equal(again[-2], x_out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for i in range(3):
+        captured[-1].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured[-1], z) and torch.equal(captured[-2], x_out)
+        step()                                                              # eager work between the replays
+        torch.cuda.synchronize()

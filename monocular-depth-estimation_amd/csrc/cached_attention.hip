@@ -17,7 +17,8 @@ struct Plan {
 // workgroups that a CU holds at once (three, two for wide heads) are there.
 // Measured, us of the first kernel / the second, 8 heads of 64 in IEEE half: 32 rows over 8192 keys 20 / 25, 96 rows 27 / 26; 384 rows
 // over 2048 keys 16 / 23; 8 sequences over 2048 keys, 96 rows 23 / 26, 256 rows 40 / 38; 64 sequences over 512 keys, 32 rows
-// 18 / 22, 64 rows 30 / 23.  Heads of 128: 8 sequences over 2048 keys, 64 rows 21 / 32, 96 rows 37 / 34; over 512 keys, 384 rows 46 / 25.
+// 18 / 22, 64 rows 30 / 23.  Heads of 128, in half and in fp32: 8 sequences over 2048 keys, 64 rows 21 / 32 and 26 / 41, 96 rows
+// 37 / 34 and 46 / 44; over 512 keys, 384 rows 46 / 25 and 58 / 38.
 constexpr int FEW_ROWS = 32, FEW_KEYS = 4096;
 constexpr int ONE_FEW = 2048, MIN_FEW = 512, MIN_MANY = 512;
 int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int heads, Plan* p) {
@@ -25,12 +26,13 @@ int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int head
     if (seqs <= 0 || max_pages <= 0 || max_q <= 0 || heads <= 0) return VDA_EINVAL;
     if (heads % c->kv_heads != 0 || (long)max_pages * c->page_size > 0x40000000L) return VDA_ESHAPE;
     const long rows = (long)max_q * (heads / c->kv_heads), keys = (long)max_pages * c->page_size;
+    if (rows > 0x3fffffffL || (long)seqs * c->kv_heads > 0x3fffffffL) return VDA_ESHAPE;
     const long few_items = (rows + 15) / 16 * seqs * c->kv_heads;
-    const bool few = rows <= FEW_ROWS || (keys <= FEW_KEYS && few_items <= ((c->hd <= 64 ? 3L : 2L) << 18) / keys);
+    const bool few = rows <= FEW_ROWS || (keys <= FEW_KEYS && few_items <= ((c->hd <= 64 ? 6L : 5L) << 17) / keys);
     p->block_rows = few ? 16 : 128;
     p->hd_pad = (c->hd + 31) & ~31;
     const long blocks = (rows + p->block_rows - 1) / p->block_rows, items = blocks * seqs * c->kv_heads;
-    if (rows > 0x3fffffffL || items > 0x3fffffffL) return VDA_ESHAPE;
+    if (items > 0x3fffffffL) return VDA_ESHAPE;
     long chunk = keys;                                            // keys of a part, a multiple of 32 for each of eight waves
     if (few) {
         p->waves = items >= 4096 || keys <= 64 ? 1 : 8;
@@ -47,11 +49,11 @@ int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int head
     }
     chunk = (chunk + 255) & ~255L;
     const long splits = (keys + chunk - 1) / chunk;
+    if (items * splits > 0x7fffffffL) return VDA_ESHAPE;
     p->chunk = (int)chunk;
     p->splits = (int)splits;
     p->row_blocks = (int)blocks;
     p->work = p->splits == 1 ? 0 : items * p->splits * p->block_rows * (p->hd_pad + 2) * (long)sizeof(float);
-    if (items * p->splits > 0x7fffffffL) return VDA_ESHAPE;
     return VDA_OK;
 }
 

@@ -226,3 +226,11 @@ def test_argument_structs_match_the_header(tmp_path):
     got = [int(v) for v in subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.split()]
     of = {"VdaTokenCache": hip.CacheDesc, "VdaCachedAttentionArgs": hip.CachedAttentionArgs, "VdaGatedNormArgs": hip.GatedNormArgs}
     assert got == [getattr(of[n], f).offset for n, f in fields] + [ctypes.sizeof(s) for s in of.values()]
+
+
+def test_c_attention_refuses_sizes_beyond_its_counters():
+    n = hip.lib().vda_cached_attention_work
+    big = (1 << 31) - 1
+    for seqs, max_pages, max_q, heads in ((1, 4, big, 4), (big, 4, 1, 4), (big, 4, big, 4), (big, 1 << 20, big, big // 2 * 2), (1, (1 << 30) // 32 + 1, 1, 4)):
+        assert n(ctypes.byref(desc()), seqs, max_pages, max_q, heads) == ESHAPE, (seqs, max_pages, max_q, heads)
+    assert n(ctypes.byref(desc()), 1, (1 << 30) // 32, 1, 4) > 0

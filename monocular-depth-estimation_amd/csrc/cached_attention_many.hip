@@ -6,8 +6,8 @@
 // query lives on a lane, the softmax needs one exchange (lane ^ 32) and only where a maximum grows, and the probabilities
 // are as they stand the B operand of O^T += V^T P^T, whose V^T operand the transposed LDS read gathers in the same key order.
 // What bounds it is vector instruction issue: about five instructions per score, one of them the exponential, against two matrix
-// instructions of 32 cycles per 1024 scores and 16 channels.  The 1370 tokens of a frame over 32 frames, 16 heads of 64: 375 us,
-// 0.66 PFLOP/s, where a large library product of the type reaches 1.2.  Vector and matrix instructions of different waves take
+// instructions of 32 cycles per 1024 scores and 16 channels.  The 1370 tokens of a frame over 32 frames, 16 heads of 64: 375 us
+// (416 on a slower card), 0.66 PFLOP/s, where a large library product of the type reaches 1.2.  Vector and matrix instructions of different waves take
 // turns at the issue, so a fourth wave per SIMD (32 keys per tile) gains nothing: 388 us.  Within a wave, the scores of one half of the
 // tile formed between the exponentials of the other: 1 % less here, 3 % more for three clips of 5 x 380 tokens, not kept; the
 // scores of the next tile between them: 204 registers, two waves, 607 us.  64 rows per wave: slower.

@@ -89,6 +89,7 @@ extern "C" int vda_cached_attention(const VdaTokenCache* cache, const VdaCachedA
     const int size = a->dtype == VDA_T_F32 ? 4 : 2;
     if (a->ldq < (long)a->heads * cache->hd || a->ldo < (long)a->heads * cache->hd || a->rows > 0x7fffffffL) return VDA_ESHAPE;
     if ((((uintptr_t)a->q | (uintptr_t)a->out) & 15) != 0 || (a->ldq * size) % 16 != 0 || (a->ldo * size) % 16 != 0) return VDA_ESHAPE;
+    if (a->q == a->out && a->ldq != a->ldo) return VDA_EINVAL;
     if (p.work > 0) {
         if (!a->work) return VDA_EINVAL;
         if (a->work_bytes < p.work || ((uintptr_t)a->work & 15) != 0) return VDA_ESHAPE;

@@ -565,6 +565,20 @@ def test_attention_graphs_on_two_streams_with_workspaces_of_their_own(q_len, kv)
             assert torch.equal(got, w)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("q_len,kv,table_pages", [(1, 40, 3), (5, 700, 44), (3, 6000, 375), (150, 700, 300)])
+def test_attention_in_place_of_its_queries(q_len, kv, table_pages, dt):
+    m = Memory([kv, 33], 2, 64, 16, "i8", 141)
+    m.table = torch.nn.functional.pad(m.table, (0, table_pages - m.table.shape[1]), value=-1)
+    q = queries(2 * q_len, 4, 64, dt, 142)
+    start = torch.tensor([0, q_len, 2 * q_len], dtype=torch.int32, device=DEV)
+    kw = dict(heads=4, kv_heads=2, hd=64, page_size=16, fmt=hip.CACHE_I8, max_q=q_len, scale=0.125)
+    out = torch.empty_like(q)
+    hip.cached_attention(q, out, *m.planes, m.table.to(DEV), m.kv_len.to(DEV), start, **kw)
+    hip.cached_attention(q, q, *m.planes, m.table.to(DEV), m.kv_len.to(DEV), start, **kw)
+    assert torch.equal(q, out)
+
+
 # ---- the operators together ----------------------------------------------------------------------------------------------------------
 def product_check(got, a, w):
     """A product of 16-bit operands with fp32 sums, rounded to got's type."""

@@ -243,3 +243,8 @@ def test_c_cache_refuses_key_heads_that_overflow_a_workgroups_count():
     assert hip.lib().vda_cache_write(ctypes.byref(d), A, A, A, 1, row, row, hip.T_F16, None, None, 0, 0, 0, 0, 0, None) == ESHAPE
     assert hip.lib().vda_cache_read(ctypes.byref(d), A, A, A, 1, row, row, hip.T_F16, None) == ESHAPE
     assert hip.lib().vda_cached_attention_work(ctypes.byref(desc(pages=1, page_size=16, kv_heads=65537)), 1, 1, 1, 65537) == ESHAPE
+
+
+def test_c_attention_in_place_needs_one_stride():
+    f = hip.lib().vda_cached_attention
+    assert f(ctypes.byref(desc()), ctypes.byref(attention_args(q=A, out=A, ldq=256, ldo=264)), None) == EINVAL

@@ -51,10 +51,11 @@ __device__ __forceinline__ void normalise(f32x4 (&v)[N], int kind, int lane0, in
     for (int i = 0; i < N; ++i) v[i] *= rstd;
 }
 
-// W waves share a row of up to 256 N W channels; a workgroup of four waves holds 4 / W rows.
+// W waves share a row of up to 256 N W channels: a workgroup holds four rows of one wave each, or one row.  N = 8 takes 190 registers, two
+// waves per SIMD: 20000 rows of 2048 channels, norms before and after, 243 us with one wave to a row, 114 with four and N = 2.
 template <typename TB, typename TY, int N, int W>
-__global__ __launch_bounds__(256) void gated_norm_kernel(NormArgs a, const TB* __restrict__ b, TY* __restrict__ y) {
-    __shared__ float scratch[4];
+__global__ __launch_bounds__(W == 8 ? 512 : 256) void gated_norm_kernel(NormArgs a, const TB* __restrict__ b, TY* __restrict__ y) {
+    __shared__ float scratch[W];
     const int lane0 = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
     const long row = W == 1 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long)blockIdx.x;
     if (row >= a.rows) return;
@@ -104,16 +105,16 @@ __global__ __launch_bounds__(256) void gated_norm_kernel(NormArgs a, const TB* _
 
 template <typename TB, typename TY>
 int launch(const NormArgs& a, const void* b, void* y, hipStream_t st) {
-    const int wave_row = a.C <= 2048;
+    const int wave_row = a.C <= 1024;
     const long grid = wave_row ? (a.rows + 3) / 4 : a.rows;
     if (grid > 0x7fffffffL) return VDA_ESHAPE;
-#define VDA_GN(N, W) hipLaunchKernelGGL((gated_norm_kernel<TB, TY, N, W>), dim3(grid), dim3(256), 0, st, a, (const TB*)b, (TY*)y)
+#define VDA_GN(N, W) hipLaunchKernelGGL((gated_norm_kernel<TB, TY, N, W>), dim3(grid), dim3(W == 8 ? 512 : 256), 0, st, a, (const TB*)b, (TY*)y)
     if (a.C <= 256) VDA_GN(1, 1);
     else if (a.C <= 512) VDA_GN(2, 1);
     else if (a.C <= 1024) VDA_GN(4, 1);
-    else if (a.C <= 2048) VDA_GN(8, 1);
+    else if (a.C <= 2048) VDA_GN(2, 4);
     else if (a.C <= 4096) VDA_GN(4, 4);
-    else VDA_GN(8, 4);
+    else VDA_GN(4, 8);
 #undef VDA_GN
     return hip_rc(hipGetLastError());
 }

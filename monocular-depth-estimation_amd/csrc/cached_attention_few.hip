@@ -61,18 +61,18 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
     // this lane's part of a V tile: it copies 16 bytes of HDP / 32 keys
     char* vt = smem + wave * (32 * HDP);
     int v_key[CB], v_lds[CB];
-    unsigned v_off[CB], k_off[C64 + TAIL32];                        // bytes from a block's first row
+    int v_col[CB], k_col[C64 + TAIL32];                             // bytes of a row
 #pragma unroll
     for (int i = 0; i < CB; ++i) {
         const int idx = i * 64 + lane;
         v_key[i] = idx / (HDP / 16);
         const int col = (idx % (HDP / 16)) * 16;
-        v_off[i] = (v_key[i] & 15) * j.row_bytes + min(col, j.row_bytes - 16);
+        v_col[i] = min(col, j.row_bytes - 16);
         v_lds[i] = vtile<HDP>(v_key[i], col);
     }
 #pragma unroll
-    for (int i = 0; i < C64; ++i) k_off[i] = c16 * j.row_bytes + min(64 * i + 16 * g, j.row_bytes - 16);
-    if (TAIL32) k_off[C64] = c16 * j.row_bytes + min(64 * C64 + 8 * g, j.row_bytes - 8);
+    for (int i = 0; i < C64; ++i) k_col[i] = min(64 * i + 16 * g, j.row_bytes - 16);
+    if (TAIL32) k_col[C64] = min(64 * C64 + 8 * g, j.row_bytes - 8);
 
     // A step has two blocks of 16 keys, each in one page (a page holds a multiple of 16 slots); a block without one reads as empty
     // slots.  Pages are asked for one step ahead, from constant memory: scalar loads, for which no other load has to be waited.
@@ -99,8 +99,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
         }
     };
     ask();
-    auto fetch = [&](Step<HDP>& st) {
+    const Span sp = span_of(j, s, max_q);
+    auto fetch = [&](Step<HDP>& st, int k0) {
         long r[2];
+        int last[2];                                                // of a block's rows; those behind the sequence's last key are not read from memory
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const bool any = page[b] >= 0 && page[b] < j.pages;
@@ -108,9 +110,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
             // (global memory, said aloud, with scalar bases and 32-bit offsets of the lanes)
             global kr = (global)(j.k + r[b] * j.row_bytes), ke = (global)(j.k_exp + r[b]), ve = (global)(j.v_exp + r[b]);
             asm("" : "+s"(kr), "+s"(ke), "+s"(ve));
+            last[b] = max(0, sp.n - 1 - k0 - 16 * b);
+            const unsigned at = min(c16, last[b]) * j.row_bytes;
 #pragma unroll
-            for (int i = 0; i < C64; ++i) st.k[b][i] = *(global16)(kr + k_off[i]);
-            if (TAIL32) st.k8[b] = *(global8)(kr + k_off[C64]);
+            for (int i = 0; i < C64; ++i) st.k[b][i] = *(global16)(kr + (at + k_col[i]));
+            if (TAIL32) st.k8[b] = *(global8)(kr + (at + k_col[C64]));
             st.ek[b] = *(global4)(ke + 4u * g);
             st.ev[b] = *(global4)(ve + 4u * g);
             if (!any) st.ek[b] = 0u;
@@ -119,18 +123,18 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
         asm("" : "+s"(vr[0]), "+s"(vr[1]));
 #pragma unroll
         for (int i = 0; i < CB; ++i) {
-            if (HDP % 64 == 0) st.v[i] = *(global16)(vr[2 * i / CB] + v_off[i]);       // (a block's keys fill whole chunks of 64 lanes)
-            else st.v[i] = *(global16)((v_key[i] < 16 ? vr[0] : vr[1]) + v_off[i]);
+            const unsigned at = min(v_key[i] & 15, HDP % 64 == 0 ? last[2 * i / CB] : v_key[i] < 16 ? last[0] : last[1]) * j.row_bytes + v_col[i];
+            if (HDP % 64 == 0) st.v[i] = *(global16)(vr[2 * i / CB] + at);       // (a block's keys fill whole chunks of 64 lanes)
+            else st.v[i] = *(global16)((v_key[i] < 16 ? vr[0] : vr[1]) + at);
         }
         next_block(1, 0);
         ask();
     };
-    // the first keys are asked for before it is known whether the sequence has them (the planes hold them in any case): the loads
-    // of lengths, query rows and keys are in flight together
+    // the first keys are asked for before it is known whether a row of the block sees them: the loads of keys, limits and query rows
+    // are in flight together
     Step<HDP> now;
-    fetch(now);
+    fetch(now, k_begin);
 
-    const Span sp = span_of(j, s, max_q);
     const int rho = rb * 16 + c16, n_rho = sp.nq * j.group;
     if (rb * 16 >= n_rho || split * j.chunk >= max(sp.n, 1)) return;      // the whole workgroup
     const int token = j.by_group.over(rho), head = kvh * j.group + (rho - token * j.group);
@@ -283,7 +287,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
         }
     };
     for (int k0 = k_begin; k0 < k_end; k0 += 32) {
-        if (k0 > k_begin) fetch(now);
+        if (k0 > k_begin) fetch(now, k0);
         step(now, k0);
     }
 

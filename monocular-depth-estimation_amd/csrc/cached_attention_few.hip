@@ -371,16 +371,25 @@ __global__ __launch_bounds__(256) void attend_join_kernel(T* __restrict__ out, A
     const int parts = max(1, (sp.n + j.chunk - 1) / j.chunk);
     float m = LOWEST, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int x = 0; x < parts; ++x) {
-        const float* px = p + x * stride;
-        const float mx = px[block_rows * hdp + r], lx = px[block_rows * hdp + block_rows + r];
-        const f32x4 ox = *reinterpret_cast<const f32x4*>(px + r * hdp + d);
-        if (lx == 0.f) continue;
-        const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(mx - mn);
-        m = mn;
-        l = a * l + b * lx;
-        o = a * o + b * ox;
+    for (int x0 = 0; x0 < parts; x0 += 4) {                         // four parts' loads in flight together
+        float mx[4], lx[4];
+        f32x4 ox[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* px = p + min(x0 + i, parts - 1) * stride;
+            mx[i] = px[block_rows * hdp + r];
+            lx[i] = x0 + i < parts ? px[block_rows * hdp + block_rows + r] : 0.f;
+            ox[i] = *reinterpret_cast<const f32x4*>(px + r * hdp + d);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                               // (a part without a key of the row: its outputs and maximum may be anything)
+            const bool none = lx[i] == 0.f;
+            const float mn = none ? m : fmaxf(m, mx[i]), a = __builtin_amdgcn_exp2f(m - mn), b = none ? 0.f : __builtin_amdgcn_exp2f(mx[i] - mn);
+            m = mn;
+            l = a * l + b * lx[i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = a * o[k] + (none ? 0.f : b * ox[i][k]);
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int rho = rb * block_rows + r, token = j.by_group.over(rho);

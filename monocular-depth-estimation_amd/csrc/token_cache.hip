@@ -19,9 +19,11 @@ __device__ __forceinline__ float2 turn(const Axes& a, long row, int j) {
     const double p = a.pos_float ? (double)reinterpret_cast<const float*>(a.pos)[at] : (double)reinterpret_cast<const int*>(a.pos)[at];
     double rev = p * a.freq[j] * 0.15915494309189533577;
     rev -= rint(rev);
+    const float f = (float)(2.0 * rev);                           // in half turns; what its rounding leaves out turns the result a little further
+    const float d = (float)((2.0 * rev - (double)f) * 3.14159265358979323846);
     float2 cs;
-    sincospif((float)(2.0 * rev), &cs.y, &cs.x);
-    return cs;
+    sincospif(f, &cs.y, &cs.x);
+    return float2{fmaf(-cs.y, d, cs.x), fmaf(cs.x, d, cs.y)};
 }
 
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };

@@ -23,10 +23,10 @@ constexpr int MIN_PART = 512;        // keys of a part at least
 
 // Keys of a part, for workgroups of eight waves and `items` of them per part.  A workgroup costs its keys and what 700 more would
 // (first loads, join of the waves); up to 256 run side by side, one on each CU, and 512 take half as long again (wide heads, whose
-// registers leave room for one on a CU: twice as long).  The join of the parts costs as 2000 keys: 5 us on the device, and a second launch.
+// registers leave room for one on a CU: twice as long).  The join of the parts costs as 2000 keys: 4 us on the device, and a second launch.
 // Tried: parts that make 256, 512, ... 2048 workgroups.  Measured, us of 1 part / 512 / 1024 / 2048 workgroups on the device, heads of 64:
 // 64 items of 10960 keys 60 / 28 / 35 / 40, 192 items 71 / 61 / 58 / 62, 256 items of 4096 keys 29 / 31 / 34 / 41, 512 items of 10960
-// keys 147 / - / 155 / 159; 6 items of 3000 keys 18.8, in six parts 12.3; heads of 128: 192 items of 10960 keys 114 / 132 / 126 / 137.
+// keys 147 / - / 155 / 159; 6 items of 3000 keys 18.8, in six parts 10.1; heads of 128: 192 items of 10960 keys 114 / 132 / 126 / 137.
 long part_of(long keys, long items, bool wide) {
     long best = 0, part = keys;
     for (int j = 0; j <= 8; ++j) {

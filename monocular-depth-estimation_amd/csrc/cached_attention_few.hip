@@ -11,7 +11,7 @@
 // overlap.
 //
 // Measured: one token for each of 48 streams over one to eight frames of 1370 tokens, 16 query heads on 4 key heads of 64 (170 MB),
-// 42 us here, 4.0 TB/s, and 5.7 us in the join; one token for each of 5476 positions over 32 keys, 8 heads of 32 (98 MB), 29 us,
+// 41 us here, 4.1 TB/s, and 4.7 us in the join; one token for each of 5476 positions over 32 keys, 8 heads of 32 (98 MB), 29 us,
 // 3.4 TB/s: there a wave lives for one step and its chain of loads (arguments, page, keys) is what it lasts.
 #include "cached_attention.h"
 
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
 }
 
 // The parts of a row block joined in their order: out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, the maximum m found on the way.
-// A thread per row and four channels; grid (item, run of rows).
+// A thread per row and four channels; grid (item, run of rows).  Latency bound: with one part's loads at a time 42 parts took 14 us longer.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(T* __restrict__ out, AttendJob j, int max_q, int block_rows, int hdp) {
     const int item = blockIdx.x, t0 = j.by_heads.over(item), kvh = item - t0 * j.kv_heads, s = j.by_blocks.over(t0), rb = t0 - s * j.row_blocks;

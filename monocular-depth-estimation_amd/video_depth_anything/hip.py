@@ -615,22 +615,46 @@ def _here(what, *ts):
 
 
 def _rows(what, name, t, rows, width, ld):
-    """(address, elements from one row to the next) of ``rows`` rows of ``width`` dense values: the stride is ``ld``, or what the
-    tensor's own says, and the tensor's memory holds them."""
+    """(address, elements from one row to the next) of ``rows`` rows of ``width`` dense values.  A given ``ld`` counts from the
+    tensor's first element.  Otherwise the tensor says where the rows lie: they are its first axis, whose other axes are dense and
+    hold a row (or more: its leading values), or all of its leading axes where these follow each other at one distance."""
     if ld is None and t.is_contiguous() and t.numel() == rows * width:
         return t.data_ptr(), width
-    if t.dim() >= 2:
-        dense = 1
-        for n, s in zip(t.shape[:0:-1], t.stride()[:0:-1]):
-            if n != 1 and s != dense:
-                raise ValueError(f"{what}: the rows of {name} are not dense (strides {tuple(t.stride())})")
-            dense *= n
-        if ld is None:
-            ld = max(t.stride(0), width) if t.shape[0] > 1 else width
-    elif ld is None:
-        ld = width
+    shape, strides = t.shape, t.stride()
+    dense, i = 1, t.dim()
+    while i and dense < width:                              # the last axes, up to where they hold a row
+        i -= 1
+        if shape[i] != 1 and strides[i] != dense:
+            raise ValueError(f"{what}: the rows of {name} are not dense (shape {tuple(shape)}, strides {strides})")
+        dense *= shape[i]
+    if ld is None:
+        if i == 0:                                          # dense as a whole
+            have, ld = dense // width if t.dim() == 1 or dense == width else 0, width
+        elif shape[0] == rows and all(n == 1 or s == d for n, s, d in zip(shape[1:i], strides[1:i], _dense_strides(shape, i))):
+            have, ld = rows, strides[0] if rows > 1 else width
+        else:
+            outer = [(n, s) for n, s in zip(shape[:i], strides[:i]) if n != 1] or [(1, width)]
+            have, ld = outer[-1]
+            for n, s in outer[-2::-1]:
+                if s != ld * have:
+                    raise ValueError(f"{what}: the rows of {name} lie at different distances (shape {tuple(shape)}, strides {strides})")
+                have *= n
+            if dense != width or (have > rows and len(outer) > 1):
+                have = 0
+        if rows > 1 and ld < width:
+            raise ValueError(f"{what}: the rows of {name} overlap (shape {tuple(shape)}, strides {strides})")
+        if have < rows:
+            raise ValueError(f"{what}: {name} holds other rows than {rows} of {width} (shape {tuple(shape)}, strides {strides})")
     _need(what, **{name: (t, (rows - 1) * ld + width)})
     return t.data_ptr(), ld
+
+
+def _dense_strides(shape, i):
+    """The strides that axes 1 .. i - 1 have where all axes behind the first one are dense."""
+    d = [1]
+    for n in shape[:0:-1]:
+        d.append(d[-1] * n)
+    return d[-2:-i - 1:-1]
 
 
 def _vector(what, name, t, elements, dtype):

@@ -248,3 +248,87 @@ def test_c_cache_refuses_key_heads_that_overflow_a_workgroups_count():
 def test_c_attention_in_place_needs_one_stride():
     f = hip.lib().vda_cached_attention
     assert f(ctypes.byref(desc()), ctypes.byref(attention_args(q=A, out=A, ldq=256, ldo=264)), None) == EINVAL
+
+
+@pytest.fixture
+def addressed(monkeypatch):
+    """The wrappers with the library replaced by a recorder of the arguments that reach it."""
+    calls = []
+
+    class Recorder:
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, a)) or 0
+
+    monkeypatch.setattr(hip, "lib", lambda: Recorder())
+    monkeypatch.setattr(hip, "_dev", lambda *ts: None)
+    monkeypatch.setattr(hip, "_current_device", lambda: -1)
+    monkeypatch.setattr(hip, "_stream", lambda: None)
+    return calls
+
+
+ROWS, HEADS, HD = 6, 4, 64
+WIDTH = HEADS * HD
+# (name, rows of WIDTH values in a tensor whose own strides say where each lies, the stride of a row)
+ROW_VIEWS = [("dense", lambda: torch.zeros(ROWS, HEADS, HD), WIDTH), ("flat", lambda: torch.zeros(ROWS * WIDTH), WIDTH), ("frames", lambda: torch.zeros(2, 3, WIDTH), WIDTH),
+             ("half rows", lambda: torch.zeros(2 * ROWS, WIDTH // 2), WIDTH), ("columns", lambda: torch.zeros(ROWS, 3 * WIDTH)[:, WIDTH:2 * WIDTH], 3 * WIDTH),
+             ("columns of frames", lambda: torch.zeros(2, 3, 3 * WIDTH)[..., WIDTH:2 * WIDTH], 3 * WIDTH), ("part of packed rows", lambda: torch.zeros(ROWS, 3, HEADS, HD)[:, 1], 3 * WIDTH),
+             ("wider rows", lambda: torch.zeros(ROWS, 2 * WIDTH), 2 * WIDTH), ("every other row", lambda: torch.zeros(2 * ROWS, WIDTH)[::2], 2 * WIDTH),
+             ("a longer buffer", lambda: torch.zeros(ROWS + 2, 2 * WIDTH)[:, :WIDTH], 2 * WIDTH), ("a longer flat one", lambda: torch.zeros(ROWS * WIDTH + 8), WIDTH)]
+# the same count of elements behind the first one, but no such rows
+NO_ROW_VIEWS = [("one row repeated", lambda: torch.zeros(16, WIDTH)[2:3].expand(ROWS, WIDTH)), ("one row of heads repeated", lambda: torch.zeros(16, HEADS, HD)[2:3].expand(ROWS, HEADS, HD)),
+                ("heads apart", lambda: torch.zeros(ROWS * HEADS, 2 * HD)[:, :HD]), ("overlapping windows", lambda: torch.zeros(16 * WIDTH).as_strided((ROWS, WIDTH), (64, 1))),
+                ("frames apart", lambda: torch.zeros(8, 4, WIDTH)[:2, 1:]), ("rows of frames, more of them", lambda: torch.zeros(8, 4, WIDTH)),
+                ("a strided line", lambda: torch.zeros(4 * ROWS * WIDTH)[::2]), ("packed rows taken for rows", lambda: torch.zeros(ROWS + 1, 3, WIDTH)),
+                ("turned", lambda: torch.zeros(16 * WIDTH, 16).t()[:ROWS, :WIDTH]), ("a shorter view of a longer buffer", lambda: torch.zeros(16, WIDTH)[:ROWS - 1]),
+                ("a shorter line of a longer buffer", lambda: torch.zeros(16 * WIDTH)[:ROWS * WIDTH - 1])]
+
+
+def row_calls(addressed):
+    """For each wrapper and each of its row operands: a call with that operand given, and where its stride is found."""
+    f = f16
+    pos, freq, slots = torch.zeros(ROWS, 3, dtype=i32), torch.zeros(32, dtype=f64), torch.zeros(ROWS, dtype=i64)
+    p = planes(heads=HEADS, hd=HD)
+    seq = torch.zeros(1, 3, dtype=i32), torch.zeros(1, dtype=i32), torch.zeros(2, dtype=i32)
+    good = lambda t=f: torch.zeros(ROWS, WIDTH, dtype=t)  # noqa: E731
+    rot, cache = dict(rows=ROWS, heads=HEADS, hd=HD, sections=(8, 12, 12)), dict(rows=ROWS, kv_heads=HEADS, hd=HD, page_size=16, fmt=hip.CACHE_I8)
+    att = dict(heads=HEADS, kv_heads=HEADS, hd=HD, page_size=16, fmt=hip.CACHE_I8, max_q=ROWS, scale=0.1, rows=ROWS)
+    norm = lambda x=None, b=None, x_out=None, y=None: hip.gated_norm(good(f32) if x is None else x, good() if b is None else b, good(f32) if x_out is None else x_out,  # noqa: E731
+                                                                     good() if y is None else y, rows=ROWS, C=WIDTH)
+    arg = lambda i: lambda: addressed[-1][1][i]  # noqa: E731
+    field = lambda name, which: lambda: getattr(which.from_buffer_copy(addressed[-1][1][1 if which is hip.CachedAttentionArgs else 0]), name)  # noqa: E731
+    return [(f, lambda t: hip.rotary_axes(t, good(), pos, freq, **rot), arg(7)), (f, lambda t: hip.rotary_axes(good(), t, pos, freq, **rot), arg(8)),
+            (f, lambda t: hip.cache_write(t, good(), *p, slots, **cache), arg(5)), (f, lambda t: hip.cache_write(good(), t, *p, slots, **cache), arg(6)),
+            (f, lambda t: hip.cache_read(*p, slots, t, good(), **cache), arg(5)), (f, lambda t: hip.cache_read(*p, slots, good(), t, **cache), arg(6)),
+            (f, lambda t: hip.cached_attention(t, good(), *p, *seq, **att), field("ldq", hip.CachedAttentionArgs)),
+            (f, lambda t: hip.cached_attention(good(), t, *p, *seq, **att), field("ldo", hip.CachedAttentionArgs)),
+            (f32, lambda t: norm(x=t), field("ldx", hip.GatedNormArgs)), (f, lambda t: norm(b=t), field("ldb", hip.GatedNormArgs)),
+            (f32, lambda t: norm(x_out=t), field("ldxo", hip.GatedNormArgs)), (f, lambda t: norm(y=t), field("ldy", hip.GatedNormArgs))]
+
+
+@pytest.mark.parametrize("name,make,ld", ROW_VIEWS, ids=[v[0] for v in ROW_VIEWS])
+def test_rows_lie_where_the_tensors_strides_say(addressed, name, make, ld):
+    for dtype, call, stride in row_calls(addressed):
+        call(make().to(dtype) if make().is_contiguous() else torch.zeros(make().untyped_storage().nbytes() // 4, dtype=dtype).as_strided(make().shape, make().stride(), make().storage_offset()))
+        assert stride() == ld
+
+
+@pytest.mark.parametrize("name,make", NO_ROW_VIEWS, ids=[v[0] for v in NO_ROW_VIEWS])
+def test_tensors_whose_strides_make_no_such_rows_are_refused(addressed, name, make):
+    """Their memory reaches far enough: taken for dense rows, the call would read and write values of other rows or none."""
+    for dtype, call, _ in row_calls(addressed):
+        t = make()
+        t = torch.zeros(t.untyped_storage().nbytes() // 4, dtype=dtype).as_strided(t.shape, t.stride(), t.storage_offset())
+        with pytest.raises(ValueError):
+            call(t)
+
+
+def test_a_row_stride_that_is_given_counts_from_the_tensors_first_element(addressed):
+    pos, freq = torch.zeros(ROWS, 3, dtype=i32), torch.zeros(32, dtype=f64)
+    kw = dict(rows=ROWS, heads=HEADS, hd=HD, sections=(8, 12, 12))
+    out, buf = torch.zeros(ROWS, WIDTH, dtype=f16), torch.zeros(ROWS * 3 * WIDTH, dtype=f16)
+    for t in (buf, buf[WIDTH:], buf.view(ROWS, 3, HEADS, HD)[:, 1], buf.view(1, ROWS, 3 * WIDTH)[..., :WIDTH]):
+        hip.rotary_axes(t, out, pos, freq, ldx=3 * WIDTH, **kw)
+        assert addressed[-1][1][7] == 3 * WIDTH
+    for bad in (buf[2 * WIDTH + 8:], torch.zeros(8 * ROWS, 2 * HD, dtype=f16)[:, :HD]):          # beyond the memory; a row that is not dense
+        with pytest.raises(ValueError):
+            hip.rotary_axes(bad, out, pos, freq, ldx=3 * WIDTH, **kw)

@@ -7,8 +7,12 @@
 // 4g .. 4g+3 (g = lane / 16) of two blocks of 16, which, exponentiated, is the B operand of O^T = V^T P^T if the 8 keys of lane group g
 // are taken in that order.  V^T needs 8 keys of one channel per lane: the codes pass through LDS, whose transposed
 // 16-bit read delivers pairs of channels, even and odd channels becoming two operands.  A value's exponent multiplies its
-// probability (relative to the largest exponent so far), so codes are never scaled.  Loads and products of different waves
-// overlap.
+// probability, so codes are never scaled.  Loads and products of different waves overlap.
+//
+// What becomes a half is the probability times the value's power of two, so what a row is taken relative to is the largest sum of
+// score and value exponent, in octaves, of the keys that this row sees and weighs: large values of keys that it does not see, or
+// gives no weight, cost it no bits.  A row's reference moves when its own scores ask for it, never for another row's sake: its bits do not
+// depend on what its neighbours see.
 //
 // Measured: one token for each of 48 streams over one to eight frames of 1370 tokens, 16 query heads on 4 key heads of 64 (170 MB),
 // 41 us here, 4.1 TB/s, and 4.7 us in the join; one token for each of 5476 positions over 32 keys, 8 heads of 32 (98 MB), 29 us,
@@ -27,7 +31,8 @@ __device__ __forceinline__ int vtile(int key, int col) {
     return key * HDP + (col ^ swz);
 }
 
-constexpr int V_REF_MIN = 40;        // smallest reference of the value exponents: values of 1e-33 and less lose bits against it
+constexpr float V_REF_MIN = 40.f;    // a smaller value exponent counts as this one in the reference, or the sum of the probabilities would
+                                     // overflow: values of 1e-31 and less lose bits
 
 template <int HDP> struct Step {
     u32x4 k[2][HDP >= 64 ? HDP / 64 : 1];         // 64 channels of a key: 16 bytes per lane
@@ -178,10 +183,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
     f32x4 o[CB][2];
 #pragma unroll
     for (int i = 0; i < CB; ++i) { o[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; o[i][1] = o[i][0]; }
-    // m_run: largest score so far in octaves.  Values' exponents are relative to v_ref, the largest so far (the same in every lane):
-    // probabilities, their sum and the outputs all carry the factor 2^(127 + P_SHIFT - v_ref), which cancels in the end
+    // m_run: largest score plus value exponent so far, in octaves.  Probabilities, their sum and the outputs all carry the factor
+    // 2^(127 + P_SHIFT - m_run), which cancels in the end
     float m_run = LOWEST, l_run = 0.f;
-    int v_ref = V_REF_MIN;
 
     auto step = [&](Step<HDP>& st, int k0) {
         // V codes to LDS (in the order of the keys); the wave alone reads them, LDS operations of a wave stay in order
@@ -209,15 +213,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
 #pragma unroll
             for (int i = 0; i < 4; ++i) sc[b][i] = a[i] * power_of_byte(byte_of(st.ek[b], i));
         }
-        int top = 0;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = max(top, (int)byte_of(st.ev[b], i));
         // what is not seen: keys beyond the row's limit, empty slots; what is seen and not a number: rows with exponent 255
         unsigned keep[2] = {0xffffffffu, 0xffffffffu};
-        if (__builtin_amdgcn_ballot_w64((odd_bytes(st.ek[0]) | odd_bytes(st.ek[1])) != 0 || top == 255 || k0 + 32 > limit) != 0) {
-            top = 0;
+        if (__builtin_amdgcn_ballot_w64((odd_bytes(st.ek[0]) | odd_bytes(st.ek[1]) | odd_bytes(st.ev[0]) | odd_bytes(st.ev[1])) != 0 || k0 + 32 > limit) != 0) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 keep[b] = 0u;
@@ -230,7 +228,6 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
                     if (there && !nan) {
                         keep[b] |= 255u << (8 * i);
                         ev |= w << (8 * i);
-                        top = max(top, (int)w);
                     }
                     if (!there || key >= limit) sc[b][i] = -INFINITY;
                     else if (nan) sc[b][i] = __builtin_nanf("");
@@ -238,22 +235,23 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
                 st.ev[b] = ev;
             }
         }
-        float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * c_row;
-        if (__builtin_amdgcn_ballot_w64(mx > m_run + DEFER || top > v_ref) != 0) {
+        float mx = LOWEST;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaf(sc[b][i], c_row, fmaxf((float)byte_of(st.ev[b], i), V_REF_MIN)));
+        if (__builtin_amdgcn_ballot_w64(mx > m_run + DEFER) != 0) {
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            top = max(top, __shfl_xor(top, 16));
-            top = max(top, __shfl_xor(top, 32));
-            const float m_new = fmaxf(m_run, mx);
-            const int ref = max(v_ref, top);
-            const float alpha = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(m_run - m_new), v_ref - ref);
-            l_run *= alpha;
+            const float m_new = mx > m_run + DEFER ? mx : m_run;
+            // in two steps: where a value exponent grew by more than 126, the factor's square is below the smallest number and the sum is not
+            const float root = __builtin_amdgcn_exp2f(0.5f * (m_run - m_new)), alpha = root * root;
+            l_run = l_run * root * root;
 #pragma unroll
             for (int i = 0; i < CB; ++i) { o[i][0] *= alpha; o[i][1] *= alpha; }
             m_run = m_new;
-            v_ref = ref;
         }
-        const float base = (float)(127 + P_SHIFT - v_ref) - m_run;
+        const float base = (float)(127 + P_SHIFT) - m_run;
         f16x8 pf[NP];
         float sum = 0.f;
 #pragma unroll
@@ -262,7 +260,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
             for (int i = 0; i < 4; ++i) {
                 const float p = __builtin_amdgcn_exp2f(fmaf(sc[b][i], c_row, base));
                 sum += p;
-                const float w = p * power_of_byte(byte_of(st.ev[b], i));
+                const float w = p * power_of_byte(byte_of(st.ev[b], i));         // at most 2^(P_SHIFT + DEFER), rounded to 11 bits (22 in two pieces)
                 const f16 hi = (f16)w;
                 pf[0][4 * b + i] = hi;
                 if (NP == 2) pf[NP - 1][4 * b + i] = (f16)(w - (float)hi);
@@ -294,17 +292,6 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
     // lane (c16, g) holds channels 32 i + 8 g + 0..7 of query c16, even ones in o[i][0], odd ones in o[i][1]
     l_run += __shfl_xor(l_run, 16);
     l_run += __shfl_xor(l_run, 32);
-    if (W > 1) {         // parts with references of their own will meet: back to their own scale
-        const int back = v_ref - 127 - P_SHIFT;
-        l_run = __builtin_amdgcn_ldexpf(l_run, back);
-#pragma unroll
-        for (int i = 0; i < CB; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                o[i][0][x] = __builtin_amdgcn_ldexpf(o[i][0][x], back);
-                o[i][1][x] = __builtin_amdgcn_ldexpf(o[i][1][x], back);
-            }
-    }
     if constexpr (W > 1) {        // join the waves' parts: [wave][16 rows][LD] outputs, then [wave][16] maxima and sums
         __syncthreads();                                            // the V tiles are done with
         float* jo = reinterpret_cast<float*>(smem);
@@ -327,9 +314,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float a = __builtin_amdgcn_exp2f(jm[w * 16 + r] - m);
-                l += a * jm[W * 16 + w * 16 + r];
-                v += a * *reinterpret_cast<const f32x4*>(jo + (w * 16 + r) * LD + d);
+                const float root = __builtin_amdgcn_exp2f(0.5f * (jm[w * 16 + r] - m));
+                l += jm[W * 16 + w * 16 + r] * root * root;
+                v += root * root * *reinterpret_cast<const f32x4*>(jo + (w * 16 + r) * LD + d);
             }
             if (j.splits > 1) {
                 *reinterpret_cast<f32x4*>(part + r * HDP + d) = v;
@@ -384,11 +371,11 @@ __global__ __launch_bounds__(256) void attend_join_kernel(T* __restrict__ out, A
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                               // (a part without a key of the row: its outputs and maximum may be anything)
             const bool none = lx[i] == 0.f;
-            const float mn = none ? m : fmaxf(m, mx[i]), a = __builtin_amdgcn_exp2f(m - mn), b = none ? 0.f : __builtin_amdgcn_exp2f(mx[i] - mn);
+            const float mn = none ? m : fmaxf(m, mx[i]), ra = __builtin_amdgcn_exp2f(0.5f * (m - mn)), rb = none ? 0.f : __builtin_amdgcn_exp2f(0.5f * (mx[i] - mn));
             m = mn;
-            l = a * l + b * lx[i];
+            l = l * ra * ra + lx[i] * rb * rb;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = a * o[k] + (none ? 0.f : b * ox[i][k]);
+            for (int k = 0; k < 4; ++k) o[k] = ra * ra * o[k] + (none ? 0.f : rb * rb * ox[i][k]);
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -670,3 +670,94 @@ def test_a_block_over_a_memory_of_frames(dt, fmt, tokens, table_pages, pairing):
         assert torch.equal(captured[-1], z) and torch.equal(captured[-2], x_out)
         step()                                                              # eager work between the replays
         torch.cuda.synchronize()
+
+
+# ---- what a row does not see, and what it sees but does not weigh --------------------------------------------------------------------
+WIDE = [(torch.float16, "i8"), (torch.bfloat16, "e4m3"), (torch.float32, "i8"), (torch.float32, "e4m3")]
+
+
+def store(m, at, k, v):
+    """k and v ([rows, hd], for every key head) into the slots of the keys ``at``, counted over the sequences."""
+    rows = len(at)
+    wide = lambda x: x[:, None].expand(rows, m.kv_heads, m.hd).contiguous().to(DEV)  # noqa: E731
+    hip.cache_write(wide(k), wide(v), *m.planes, m.slots[at], rows=rows, kv_heads=m.kv_heads, hd=m.hd, page_size=m.page, fmt=FMT[m.fmt])
+
+
+def unseen_keys_have_no_effect(q_len, kv, first, table_pages, size, hd, dt, fmt):
+    """Every row but the last ends before key ``first``; keys from there on then become finite and very large, in the tile of the last key
+    that the rows see and behind it: no bit of those rows changes."""
+    m = Memory([kv], 2, hd, 16, fmt, 151)
+    m.table = torch.nn.functional.pad(m.table, (0, max(0, table_pages - m.table.shape[1])), value=-1)
+    visible = torch.full((q_len,), first, dtype=torch.int32)
+    visible[:q_len // 2] -= torch.arange(q_len // 2, dtype=torch.int32) % 5
+    visible[-1] = kv
+    q = queries(q_len, 4, hd, dt, 152)
+    out, want, rows = m.check(q, [0, q_len], 4, visible=visible)
+    late = list(range(first, kv))
+    one = torch.ones((len(late), hd))
+    for k, v in ((one, one * size), (one * size, one), (-one * size, one * size)):
+        store(m, late, k, v)
+        again = m.attend(q, [0, q_len], 4, visible=visible)[0]
+        assert torch.equal(again[:-1], out[:-1])
+
+
+def keys_without_weight_have_no_effect(q_len, table_pages, dt, fmt, hd=64):
+    """A key that points far away from every query has weight 0, however large it and its value are: the rows are held to the bound of
+    the memory without it."""
+    m = Memory([90], 1, hd, 16, fmt, 161)
+    m.table = torch.nn.functional.pad(m.table, (0, max(0, table_pages - m.table.shape[1])), value=-1)
+    q = queries(q_len, 2, hd, dt, 162)
+    q[..., 0] = q[..., 0].abs() + 1
+    at = 37
+    page, place = int(m.slots[at]) // 16, int(m.slots[at]) % 16
+    m.planes[2][page, :, place] = 0
+    start = torch.tensor([0, q_len], dtype=torch.int32)
+    want, tol = R.attend(q, *m.planes, m.table, m.kv_len, start, None, 2, 1, hd, 16, fmt, hd ** -0.5)
+    away = torch.zeros((1, hd))
+    for far, size in ((-2.0 ** 36, 1.0), (-2.0 ** 36, 2.0 ** 40), (-2.0 ** 14, 2.0 ** 40)):
+        away[0, 0] = far
+        store(m, [at], away, torch.ones((1, hd)) * size)
+        within(m.attend(q, [0, q_len], 2)[0], want, tol, f"key {far:.0e}, value {size:.0e}")
+
+
+def large_values_of_small_weight_count(q_len, table_pages, dt, fmt, hd=32):
+    """Values up to 2^40 times larger than the rest, on keys whose weights are as much smaller: both parts make up the output."""
+    m = Memory([200], 1, hd, 16, fmt, 171)
+    m.table = torch.nn.functional.pad(m.table, (0, max(0, table_pages - m.table.shape[1])), value=-1)
+    g = gen(172)
+    octaves = torch.randint(0, 41, (60, 1), generator=g).float()
+    k, v = torch.randn((60, hd), generator=g) * 0.1, torch.randn((60, hd), generator=g) * torch.exp2(octaves)
+    k[:, 0] = -(octaves[:, 0] * math.log(2.0) + 2) * hd ** 0.5
+    store(m, list(range(3, 183, 3)), k, v)
+    q = queries(q_len, 2, hd, dt, 173, 0.3)
+    q[..., 0] = 1.0
+    m.check(q, [0, q_len], 2)
+
+
+@pytest.mark.parametrize("dt,fmt", WIDE)
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 20, 2.0 ** 40])
+@pytest.mark.parametrize("q_len,kv,first", [(3, 90, 71), (50, 150, 100), (150, 110, 80), (4, 3000, 1300)])
+def test_attention_few_rows_unseen_keys_have_no_effect(q_len, kv, first, size, dt, fmt):
+    unseen_keys_have_no_effect(q_len, kv, first, 0, size, 64, dt, fmt)
+
+
+@pytest.mark.parametrize("dt,fmt", WIDE)
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_attention_few_rows_keys_without_weight_have_no_effect(q_len, dt, fmt):
+    keys_without_weight_have_no_effect(q_len, 0, dt, fmt)
+
+
+@pytest.mark.parametrize("dt,fmt", [(torch.bfloat16, "i8"), (torch.bfloat16, "e4m3"), (torch.float32, "i8"), (torch.float32, "e4m3")])
+@pytest.mark.parametrize("q_len,table_pages", [(1, 0), (40, 0), (1, 400)])
+def test_attention_few_rows_large_values_of_small_weight_count(q_len, table_pages, dt, fmt):
+    large_values_of_small_weight_count(q_len, table_pages, dt, fmt)
+
+
+@pytest.mark.parametrize("dt,fmt", [(torch.float16, "i8"), (torch.bfloat16, "e4m3"), (torch.float32, "i8")])
+@pytest.mark.parametrize("hd", [8, 24, 40, 48, 96, 128])
+def test_attention_few_rows_parts_joined_for_every_head_size(hd, dt, fmt):
+    """3000 keys in parts, heads that fill their padded size and heads that do not."""
+    m = Memory([3000, 40], 2, hd, 16, fmt, 181)
+    shape = dict(kv_heads=2, hd=hd, page_size=16, fmt=FMT[fmt])
+    assert hip.cached_attention_work(m.planes[0], seqs=2, max_pages=m.table.shape[1], max_q=2, heads=4, **shape) > 0
+    m.check(queries(3, 4, hd, dt, 182), [0, 2, 3], 4)

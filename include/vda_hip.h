@@ -405,11 +405,13 @@ int vda_cache_read(const VdaTokenCache* cache, const int64_t* slots, void* k, vo
  *   [seqs][max_pages]) at place i % page_size.  Row r sees
  *   the first visible[r] of its sequence's keys (int32 [rows]; NULL: all): a causal mask, by token or by frame.  Keys
  *   in empty slots and in pages outside 0 .. pages-1 (evicted ones: -1) are not seen by any row.  A row that sees no key is 0.  What
- *   is not seen has no effect, NaN included.  Query heads h * G .. h * G + G-1 use key head h, G = heads / kv_heads.
+ *   is not seen has no effect on a row, NaN and values of any size included (other rows' keys may change which way a result rounds).
+ *   Query heads h * G .. h * G + G-1 use key head h, G = heads / kv_heads.
  *   q, out: dtype BF16, F16 or F32, rows of ldq and ldo elements, 16-byte aligned (out may be q itself, with ldo == ldq, and must not
  *   overlap it otherwise); rows of no sequence are left as they were.
- *   Scores, softmax and sums are fp32 (keys beyond 1e30 overflow them).  16-bit types: products of IEEE halves, the cached values exactly and the probabilities
- *   rounded to 11 bits; F32: q and the probabilities in two pieces (22 bits).
+ *   Scores, softmax and sums are fp32 (keys beyond 1e29 overflow them, values below 1e-30 lose bits).  16-bit types: products of IEEE
+ *   halves, the cached values exactly and the probabilities rounded to 11 bits; F32: q and the probabilities in two pieces (22
+ *   bits).  Of a row's products of probability and value, what lies below 2^-25 of the largest is lost.
  *   work: vda_cached_attention_work bytes of scratch, 16-byte aligned, of no meaning between calls; calls that may run at the
  *   same time need one each.  Results are the same bits from run to run. */
 typedef struct VdaCachedAttentionArgs {

@@ -7,8 +7,9 @@
 struct AttendJob {
     const uint8_t *k, *v, *k_exp, *v_exp;
     const int *page_table, *kv_len, *q_start, *visible;
-    float* part;                // per (item, split): [rows of a block][hd padded] outputs, then their maxima and sums; unused where splits == 1.
-                                // A row without a key in the split leaves its outputs unwritten and its sum 0
+    float* part;                // per (item, split): [rows of a block][hd padded] outputs, then their references and sums (outputs over sums are the
+                                // part's result, both times 2^(127 + P_SHIFT - reference)); a part behind a sequence's last key is not written, a row
+                                // without a key in a written part has sum 0.  Unused where splits == 1
     long rows, ldq, ldo;
     int pages, page_size, kv_heads, hd, row_bytes, max_pages, group, seqs;
     int row_blocks, splits;     // blocks of query rows per (sequence, key head); parts of the key axis,

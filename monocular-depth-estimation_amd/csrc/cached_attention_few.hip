@@ -344,7 +344,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void 
     }
 }
 
-// The parts of a row block joined in their order: out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, the maximum m found on the way.
+// The parts of a row block joined in their order: out = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, m the largest reference, found on the way.
 // A thread per row and four channels; grid (item, run of rows).  Latency bound: with one part's loads at a time 42 parts took 14 us longer.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(T* __restrict__ out, AttendJob j, int max_q, int block_rows, int hdp) {
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(T* __restrict__ out, A
             ox[i] = *reinterpret_cast<const f32x4*>(px + r * hdp + d);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {                               // (a part without a key of the row: its outputs and maximum may be anything)
+        for (int i = 0; i < 4; ++i) {                               // (a part without a key of the row does not move the reference)
             const bool none = lx[i] == 0.f;
             const float mn = none ? m : fmaxf(m, mx[i]), ra = __builtin_amdgcn_exp2f(0.5f * (m - mn)), rb = none ? 0.f : __builtin_amdgcn_exp2f(0.5f * (mx[i] - mn));
             m = mn;

@@ -12,14 +12,26 @@
 // tile formed between the exponentials of the other: 1 % less here, 3 % more for three clips of 5 x 380 tokens, not kept; the
 // scores of the next tile between them: 204 registers, two waves, 607 us.  64 rows per wave: slower.
 //
-// Rows of the cache carry powers of two of any size, halves do not: the halves of a part of the key axis are relative to its
-// largest key exponent and its largest value exponent, found by a pass over the exponent bytes (a 33rd of the codes'
-// bytes) before the first tile.  A code is exact down to 2^-31 of that; below it the error is 2^-39 of the largest value.
+// Rows of the cache carry powers of two of any size, halves do not.  Where the exponents of a part's keys lie close enough together, and
+// those of its values, tiles hold halves relative to the largest of each: the smallest and the largest are found by a pass over the
+// exponent bytes (a 33rd of the codes' bytes) before the first tile.  Powers of two leave no trace in such products, so it does not
+// matter whose the largest was.  Elsewhere a workgroup takes the form of single exponents, as the kernel for few rows does: tiles hold the
+// codes as they are, a key's power of two multiplies its scores, and a value's is part of the exponent that becomes the probability,
+// so that a row is taken relative to its own largest sum of score and value exponent, whatever others see.  With a value row of zeros
+// in every part, which makes it so, the frame over 32 frames takes 21 % longer, clips 12 %.
 #include "cached_attention.h"
+
+#include <type_traits>
 
 namespace {
 
 constexpr int TK = 64;                                            // keys of a tile
+// Spreads of exponents that common references take.  Keys: codes stay exact, the smallest one times 2^-32 (e4m3: 2^-21) and the shift of
+// scaled16 being a half, 2^-24 at least.  Values: probabilities are halves down to 2^-33 of the row's largest, which is 2^-25 of it on
+// a value 2^8 larger than another.
+template <int FMT> constexpr int key_spread() { return FMT == VDA_CACHE_I8 ? 32 : 21; }
+constexpr int VALUE_SPREAD = 8;
+constexpr int V_MIN = 40;            // of single exponents, smaller ones of values count as this (see V_REF_MIN in the kernel for few rows)
 
 __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
@@ -61,13 +73,18 @@ __device__ __forceinline__ void scaled16(u32x4 w, int e, f16x8& lo, f16x8& hi) {
     hi = f16x8{h[4][0], h[4][1], h[5][0], h[5][1], h[6][0], h[6][1], h[7][0], h[7][1]};
 }
 
+// Waves per SIMD, at most a few registers spilled outside the loops.
+template <typename T, int HDP> constexpr int many_waves() { return HDP <= 64 ? 3 : HDP == 128 && Pieces<T>::n == 2 ? 1 : 2; }
+
 template <typename T, int HDP, int FMT>
-__global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void attend_many_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int groups) {
+__global__ __launch_bounds__(256, (many_waves<T, HDP>())) void attend_many_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int groups) {
     constexpr int NP = Pieces<T>::n, KS = HDP / 16, DB = HDP / 32, CPR = HDP / 16, NC = (HDP + 63) / 64, SHIFT = FMT == VDA_CACHE_I8 ? 8 : 6;
     constexpr int PLANE = TK * HDP * 2, BUF = 2 * PLANE;
     __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
     __shared__ uint8_t hide[2][TK];
-    __shared__ int wave_top[8];
+    // of the keys of a tile of single exponents: a key's power of two, a value's exponent less 127, the power of two that undoes it
+    __shared__ __attribute__((aligned(16))) float single[2][3][TK];
+    __shared__ int wave_top[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
     // row blocks of one (sequence, key head, split) follow each other on one XCD and share its copy of the keys
@@ -100,8 +117,9 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
     const int* table = j.page_table + (long)s * j.max_pages;
     // the largest exponents of the part's keys and values
     int k_ref, v_ref;
+    bool common;
     {
-        int tk = 1, tv = 1;
+        int tk = 1, tv = 1, lk = 255, lv = 255;
         for (int b = (k_begin >> 4) + tid; b * 16 < k_end; b += 256) {
             const int key = b * 16, pi = j.by_page.over(key), page = table[pi];
             if (page < 0 || page >= j.pages) continue;
@@ -110,15 +128,29 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int be = (int)byte_of(e[i >> 2], i & 3), bw = (int)byte_of(w[i >> 2], i & 3);
-                if (key + i < k_end && be != 0 && be != 255 && bw != 255) { tk = max(tk, be); tv = max(tv, bw); }
+                if (key + i < k_end && be != 0 && be != 255 && bw != 255) {
+                    tk = max(tk, be);
+                    tv = max(tv, bw);
+                    lk = min(lk, be == 1 ? 255 : be);             // (keys of zeros are exact at any scale)
+                    lv = min(lv, bw);
+                }
             }
         }
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { tk = max(tk, __shfl_xor(tk, o)); tv = max(tv, __shfl_xor(tv, o)); }
-        if (lane == 0) { wave_top[wave] = tk; wave_top[4 + wave] = tv; }
+        for (int o = 1; o < 64; o <<= 1) {
+            tk = max(tk, __shfl_xor(tk, o));
+            tv = max(tv, __shfl_xor(tv, o));
+            lk = min(lk, __shfl_xor(lk, o));
+            lv = min(lv, __shfl_xor(lv, o));
+        }
+        if (lane == 0) { wave_top[wave] = tk; wave_top[4 + wave] = tv; wave_top[8 + wave] = lk; wave_top[12 + wave] = lv; }
         __syncthreads();
         k_ref = __builtin_amdgcn_readfirstlane(max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3])));
         v_ref = __builtin_amdgcn_readfirstlane(max(max(wave_top[4], wave_top[5]), max(wave_top[6], wave_top[7])));
+        lk = __builtin_amdgcn_readfirstlane(min(min(wave_top[8], wave_top[9]), min(wave_top[10], wave_top[11])));
+        lv = __builtin_amdgcn_readfirstlane(min(min(wave_top[12], wave_top[13]), min(wave_top[14], wave_top[15])));
+        common = k_ref - lk <= key_spread<FMT>() && v_ref - lv <= VALUE_SPREAD;
+        if (!common) k_ref = v_ref = 127;
     }
 
     f16x8 qf[KS][NP];
@@ -191,7 +223,8 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
         k_next += TK;
         page = pages[min(pi, j.max_pages - 1)];
     };
-    auto store = [&](int buf) {
+    auto store = [&](int buf, auto relative) {
+        constexpr bool COMMON = decltype(relative)::value;
         char* b = smem + buf * BUF;
         bool odd = false;                                         // some key of the block is hidden or not a number
 #pragma unroll
@@ -204,8 +237,9 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             f16x8 k_lo, k_hi, v_lo, v_hi;
-            scaled16<FMT>(k_code[i], k_exp[i] - k_ref + SHIFT, k_lo, k_hi);
-            scaled16<FMT>(v_code[i], v_exp[i] - v_ref + SHIFT, v_lo, v_hi);
+            const int v_at = COMMON ? v_ref : max(v_exp[i], V_MIN);
+            scaled16<FMT>(k_code[i], SHIFT + (COMMON ? k_exp[i] - k_ref : 0), k_lo, k_hi);
+            scaled16<FMT>(v_code[i], SHIFT + v_exp[i] - v_at, v_lo, v_hi);
             if (do_k && s_on[i]) {
                 *reinterpret_cast<f16x8*>(b + s_k[i]) = k_lo;
                 *reinterpret_cast<f16x8*>(b + (s_k[i] ^ 16)) = k_hi;
@@ -226,11 +260,20 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
                     *reinterpret_cast<f16x8*>(b + s_v[i] + 16) = f16x8{};
                 }
             }
-            if (do_k && s_on[i] && s_col[i] == 0) hide[buf][16 * wave + s_key[i]] = k_exp[i] == 0;
+            if (do_k && s_on[i] && s_col[i] == 0) {
+                const int key = 16 * wave + s_key[i];
+                hide[buf][key] = k_exp[i] == 0;
+                if constexpr (!COMMON) {
+                    single[buf][0][key] = __builtin_amdgcn_ldexpf(1.f, k_exp[i] - 127);
+                    single[buf][1][key] = (float)(v_at - 127);
+                    single[buf][2][key] = __builtin_amdgcn_ldexpf(1.f, 127 - v_at);
+                }
+            }
         }
     };
 
-    // scores are formed relative to the running maximum (0 until the row has seen a key: then it moves there whatever its sign)
+    // scores (of single exponents: plus the value's) are formed relative to their running maximum (0 until the row has seen a key: then it
+    // moves there whatever its sign)
     f32x16 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i)
@@ -238,84 +281,99 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
         for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
     float m_run = 0.f, l_run = 0.f;                               // l_run: of probabilities times 2^P_SHIFT
     bool unset = true;
-    const int tq = (lane & 15) >> 2, tp = lane & 3, tcol = 2 * (16 * ((lane >> 4) & 1) + 4 * tp);
+    int at_row = r, at_half = h, at_key = (lane & 15) >> 2, at_col = 2 * (16 * ((lane >> 4) & 1) + 4 * (lane & 3));
 
-    if (k_begin < k_end) {
-        fetch();
-        store(0);
-    }
-    __syncthreads();
-    int cur = 0;
-    for (int k0 = k_begin; k0 < k_end; k0 += TK, cur ^= 1) {
-        fetch();                                                  // of the tile after this one, or of nothing
-        const char* kb = smem + cur * BUF;
-        const char* vb = kb + PLANE;
-        const unsigned long hidden = __builtin_amdgcn_ballot_w64(hide[cur][lane] != 0);
-        // 32 keys at a time: half the registers for scores and probabilities
+    auto walk = [&](auto relative) {
+        constexpr bool COMMON = decltype(relative)::value;
+        if (k_begin < k_end) {
+            fetch();
+            store(0, relative);
+        }
+        __syncthreads();
+        int cur = 0;
+        for (int k0 = k_begin; k0 < k_end; k0 += TK, cur ^= 1) {
+            fetch();                                              // of the tile after this one, or of nothing
+            const char* kb = smem + cur * BUF;
+            const char* vb = kb + PLANE;
+            const unsigned long hidden = __builtin_amdgcn_ballot_w64(hide[cur][lane] != 0);
+            // 32 keys at a time: half the registers for scores and probabilities
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
-            f32x16 sc;
+            for (int kh = 0; kh < 2; ++kh) {
+                f32x16 sc;
 #pragma unroll
-            for (int x = 0; x < 16; ++x) sc[x] = 0.f;
+                for (int x = 0; x < 16; ++x) sc[x] = 0.f;
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                const f16x8 kf = *reinterpret_cast<const f16x8*>(kb + ktile<HDP>(32 * kh + r, 2 * i + h));
+                for (int i = 0; i < KS; ++i) {
+                    const f16x8 kf = *reinterpret_cast<const f16x8*>(kb + ktile<HDP>(32 * kh + at_row, 2 * i + at_half));
 #pragma unroll
-                for (int p = NP - 1; p >= 0; --p) sc = mfma32(kf, qf[i][p], sc);
-            }
-            const unsigned gone = (unsigned)(kh ? hidden >> 32 : hidden);
-            const float base = (float)P_SHIFT - m_run;
+                    for (int p = NP - 1; p >= 0; --p) sc = mfma32(kf, qf[i][p], sc);
+                }
+                const unsigned gone = (unsigned)(kh ? hidden >> 32 : hidden);
+                const float base = (float)P_SHIFT - m_run;
+                const f32x4* mine4 = reinterpret_cast<const f32x4*>(&single[cur][0][32 * kh + 4 * at_half]);      // of this lane's keys: four at 0, 8, 16 and 24
+                if constexpr (COMMON) {
 #pragma unroll
-            for (int x = 0; x < 16; ++x) sc[x] = fmaf(sc[x], c_row, base);
-            if (gone != 0 || k0 + 32 * kh + 32 > least) {
-                const unsigned mine = gone >> (4 * h);
-                const int left = limit - (k0 + 32 * kh + 4 * h);
+                    for (int x = 0; x < 16; ++x) sc[x] = fmaf(sc[x], c_row, base);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) sc[x] = fmaf(sc[x] * mine4[2 * (x >> 2)][x & 3], c_row, base + mine4[TK / 4 + 2 * (x >> 2)][x & 3]);
+                }
+                if (gone != 0 || k0 + 32 * kh + 32 > least) {
+                    const unsigned mine = gone >> (4 * h);
+                    const int left = limit - (k0 + 32 * kh + 4 * h);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const int in32 = (x & 3) + 8 * (x >> 2);      // + 4 h
+                        if ((mine >> in32 & 1) || in32 >= left) sc[x] = -INFINITY;
+                    }
+                }
+                float mx = sc[0];
+#pragma unroll
+                for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sc[x]);
+                if (__builtin_amdgcn_ballot_w64(mx > DEFER + P_SHIFT || (unset && mx > -INFINITY)) != 0) {
+                    mx = fmaxf(mx, __shfl_xor(mx, 32)) - P_SHIFT;
+                    const float delta = !unset ? fmaxf(mx, 0.f) : mx == -INFINITY ? 0.f : mx, root = unset ? 1.f : __builtin_amdgcn_exp2f(-0.5f * delta), alpha = root * root;      // (in two steps: a value's exponent may have grown by more than 126)
+                    unset = unset && mx == -INFINITY;
+                    m_run += delta;
+                    l_run = l_run * root * root;
+#pragma unroll
+                    for (int i = 0; i < DB; ++i)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) o[i][x] *= alpha;
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) sc[x] -= delta;
+                }
+                float sum[2] = {0.f, 0.f};
+                f16x8 pf[2][NP];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const int in32 = (x & 3) + 8 * (x >> 2);      // + 4 h
-                    if ((mine >> in32 & 1) || in32 >= left) sc[x] = -INFINITY;
+                    const float p = __builtin_amdgcn_exp2f(sc[x]);
+                    sum[x & 1] = COMMON ? sum[x & 1] + p : fmaf(p, mine4[2 * (TK / 4) + 2 * (x >> 2)][x & 3], sum[x & 1]);      // (without the value's exponent)
+                    const f16 hi = (f16)p;                        // at most 2^(P_SHIFT + DEFER); rounded to 11 bits (22 in two pieces)
+                    pf[x >> 3][0][x & 7] = hi;
+                    if (NP == 2) pf[x >> 3][NP - 1][x & 7] = (f16)(p - (float)hi);
                 }
-            }
-            float mx = sc[0];
-#pragma unroll
-            for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sc[x]);
-            if (__builtin_amdgcn_ballot_w64(mx > DEFER + P_SHIFT || (unset && mx > -INFINITY)) != 0) {
-                mx = fmaxf(mx, __shfl_xor(mx, 32)) - P_SHIFT;
-                const float delta = !unset ? fmaxf(mx, 0.f) : mx == -INFINITY ? 0.f : mx, alpha = unset ? 1.f : __builtin_amdgcn_exp2f(-delta);
-                unset = unset && mx == -INFINITY;
-                m_run += delta;
-                l_run *= alpha;
+                l_run += sum[0] + sum[1];
 #pragma unroll
                 for (int i = 0; i < DB; ++i)
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) o[i][x] *= alpha;
+                    for (int x = 0; x < 2; ++x) {
+                        const int key = 32 * kh + 16 * x + 4 * at_half + at_key;
+                        const f16x4 lo = read_tr<f16>(vb + vtile<HDP>(key, 64 * i + at_col)), hi = read_tr<f16>(vb + vtile<HDP>(key + 8, 64 * i + at_col));
+                        const f16x8 vf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
-                for (int x = 0; x < 16; ++x) sc[x] -= delta;
+                        for (int p2 = NP - 1; p2 >= 0; --p2) o[i] = mfma32(vf, pf[x][p2], o[i]);
+                    }
             }
-            float sum[2] = {0.f, 0.f};
-            f16x8 pf[2][NP];
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const float p = __builtin_amdgcn_exp2f(sc[x]);
-                sum[x & 1] += p;
-                const f16 hi = (f16)p;
-                pf[x >> 3][0][x & 7] = hi;
-                if (NP == 2) pf[x >> 3][NP - 1][x & 7] = (f16)(p - (float)hi);
-            }
-            l_run += sum[0] + sum[1];
-#pragma unroll
-            for (int i = 0; i < DB; ++i)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int key = 32 * kh + 16 * x + 4 * h + tq;
-                    const f16x4 lo = read_tr<f16>(vb + vtile<HDP>(key, 64 * i + tcol)), hi = read_tr<f16>(vb + vtile<HDP>(key + 8, 64 * i + tcol));
-                    const f16x8 vf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-#pragma unroll
-                    for (int p2 = NP - 1; p2 >= 0; --p2) o[i] = mfma32(vf, pf[x][p2], o[i]);
-                }
+            store(cur ^ 1, relative);
+            __syncthreads();
         }
-        store(cur ^ 1);
-        __syncthreads();
+    };
+    if (common) {
+        walk(std::true_type{});
+    } else {
+        asm("" : "+v"(at_row), "+v"(at_half), "+v"(at_key), "+v"(at_col));      // (the addresses of one form are not kept for the other)
+        walk(std::false_type{});
     }
 
     // lane (r, h) holds channels 32 i + 8 g + 4 h + 0..3 of query r in o[i][4 g + 0..3]
@@ -325,16 +383,23 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
         float* part = j.part + ((((long)s * j.row_blocks + rb) * j.kv_heads + kvh) * j.splits + split) * (128 * (HDP + 2));
         const int in_wg = wave * 32 + r;
         float* d = part + in_wg * HDP + 4 * h;
+        // as the join expects them: outputs and sum relative to one power of two, which holds the value exponent; what its rounding leaves out
+        // (a hundred thousandth) multiplies both
+        const float v = (float)v_ref, m = unset ? LOWEST : m_run + v, v_in = m - m_run;
+        const float left = unset ? 1.f : __builtin_amdgcn_exp2f((m_run - (m - v_in)) + (v - v_in));
 #pragma unroll
         for (int i = 0; i < DB; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                f32x4 v;
+                f32x4 y;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) v[x] = __builtin_amdgcn_ldexpf(o[i][4 * g + x], v_ref - 127 - SHIFT);
-                *reinterpret_cast<f32x4*>(d + 32 * i + 8 * g) = v;
+                for (int x = 0; x < 4; ++x) y[x] = __builtin_amdgcn_ldexpf(o[i][4 * g + x] * left, -SHIFT);
+                *reinterpret_cast<f32x4*>(d + 32 * i + 8 * g) = y;
             }
-        if (h == 0) { part[128 * HDP + in_wg] = unset ? LOWEST : m_run; part[128 * HDP + 128 + in_wg] = l; }
+        if (h == 0) {
+            part[128 * HDP + in_wg] = m;
+            part[128 * HDP + 128 + in_wg] = __builtin_amdgcn_ldexpf(l * left, 127 - v_ref);
+        }
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -346,7 +411,7 @@ __global__ __launch_bounds__(256, Pieces<T>::n == 2 && HDP >= 96 ? 1 : 2) void a
             if (32 * i + 8 * g >= j.hd) continue;
             typename Vec<T>::v4 v;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) v[x] = (T)(__builtin_amdgcn_ldexpf(o[i][4 * g + x], v_ref - 127 - SHIFT) * inv);
+            for (int x = 0; x < 4; ++x) v[x] = (T)__builtin_amdgcn_ldexpf(o[i][4 * g + x] * inv, v_ref - 127 - SHIFT);
             *reinterpret_cast<typename Vec<T>::v4*>(orow + 32 * i + 8 * g) = v;
         }
 }

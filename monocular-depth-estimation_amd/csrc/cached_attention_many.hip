@@ -73,7 +73,7 @@ __device__ __forceinline__ void scaled16(u32x4 w, int e, f16x8& lo, f16x8& hi) {
     hi = f16x8{h[4][0], h[4][1], h[5][0], h[5][1], h[6][0], h[6][1], h[7][0], h[7][1]};
 }
 
-// Waves per SIMD, at most a few registers spilled outside the loops.
+// Waves per SIMD that the registers allow without spilling.
 template <typename T, int HDP> constexpr int many_waves() { return HDP <= 64 ? 3 : HDP == 128 && Pieces<T>::n == 2 ? 1 : 2; }
 
 template <typename T, int HDP, int FMT>
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256, (many_waves<T, HDP>())) void attend_many_kerne
         for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
     float m_run = 0.f, l_run = 0.f;                               // l_run: of probabilities times 2^P_SHIFT
     bool unset = true;
-    int at_row = r, at_half = h, at_key = (lane & 15) >> 2, at_col = 2 * (16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+    const int tq = (lane & 15) >> 2, tp = lane & 3, tcol = 2 * (16 * ((lane >> 4) & 1) + 4 * tp);
 
     auto walk = [&](auto relative) {
         constexpr bool COMMON = decltype(relative)::value;
@@ -297,20 +297,22 @@ __global__ __launch_bounds__(256, (many_waves<T, HDP>())) void attend_many_kerne
             const char* vb = kb + PLANE;
             const unsigned long hidden = __builtin_amdgcn_ballot_w64(hide[cur][lane] != 0);
             // 32 keys at a time: half the registers for scores and probabilities
-#pragma unroll
+            // (unrolled where the registers allow it without spilling: 3 waves per SIMD of 64 channels in two pieces)
+            constexpr int UNROLL = COMMON && (NP == 1 || HDP != 64) ? 2 : 1;
+#pragma unroll UNROLL
             for (int kh = 0; kh < 2; ++kh) {
                 f32x16 sc;
 #pragma unroll
                 for (int x = 0; x < 16; ++x) sc[x] = 0.f;
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
-                    const f16x8 kf = *reinterpret_cast<const f16x8*>(kb + ktile<HDP>(32 * kh + at_row, 2 * i + at_half));
+                    const f16x8 kf = *reinterpret_cast<const f16x8*>(kb + ktile<HDP>(32 * kh + r, 2 * i + h));
 #pragma unroll
                     for (int p = NP - 1; p >= 0; --p) sc = mfma32(kf, qf[i][p], sc);
                 }
                 const unsigned gone = (unsigned)(kh ? hidden >> 32 : hidden);
                 const float base = (float)P_SHIFT - m_run;
-                const f32x4* mine4 = reinterpret_cast<const f32x4*>(&single[cur][0][32 * kh + 4 * at_half]);      // of this lane's keys: four at 0, 8, 16 and 24
+                const f32x4* mine4 = reinterpret_cast<const f32x4*>(&single[cur][0][32 * kh + 4 * h]);      // of this lane's keys: four at 0, 8, 16 and 24
                 if constexpr (COMMON) {
 #pragma unroll
                     for (int x = 0; x < 16; ++x) sc[x] = fmaf(sc[x], c_row, base);
@@ -358,8 +360,8 @@ __global__ __launch_bounds__(256, (many_waves<T, HDP>())) void attend_many_kerne
                 for (int i = 0; i < DB; ++i)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const int key = 32 * kh + 16 * x + 4 * at_half + at_key;
-                        const f16x4 lo = read_tr<f16>(vb + vtile<HDP>(key, 64 * i + at_col)), hi = read_tr<f16>(vb + vtile<HDP>(key + 8, 64 * i + at_col));
+                        const int key = 32 * kh + 16 * x + 4 * h + tq;
+                        const f16x4 lo = read_tr<f16>(vb + vtile<HDP>(key, 64 * i + tcol)), hi = read_tr<f16>(vb + vtile<HDP>(key + 8, 64 * i + tcol));
                         const f16x8 vf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
                         for (int p2 = NP - 1; p2 >= 0; --p2) o[i] = mfma32(vf, pf[x][p2], o[i]);
@@ -369,12 +371,8 @@ __global__ __launch_bounds__(256, (many_waves<T, HDP>())) void attend_many_kerne
             __syncthreads();
         }
     };
-    if (common) {
-        walk(std::true_type{});
-    } else {
-        asm("" : "+v"(at_row), "+v"(at_half), "+v"(at_key), "+v"(at_col));      // (the addresses of one form are not kept for the other)
-        walk(std::false_type{});
-    }
+    if (common) walk(std::true_type{});
+    else walk(std::false_type{});
 
     // lane (r, h) holds channels 32 i + 8 g + 4 h + 0..3 of query r in o[i][4 g + 0..3]
     const float l = l_run + __shfl_xor(l_run, 32);

@@ -666,7 +666,7 @@ def _vector(what, name, t, elements, dtype):
     if not t.is_contiguous():
         raise ValueError(f"{what}: {name} is dense")
     if t.numel() < elements:
-        _need(what, **{name: (t, elements)})
+        raise ValueError(f"{what}: {name} holds {t.numel()} elements, the call needs {elements}")
     return t.data_ptr()
 
 
@@ -782,9 +782,9 @@ def cached_attention(q, out, ck, cv, ek, ev, page_table, kv_len, q_start, *, hea
         if work is None:
             work, have = torch.empty(n, dtype=_U8, device=q.device), n
         else:
-            have = work.untyped_storage().nbytes() - work.storage_offset() * work.element_size()
+            have = work.numel() * work.element_size() if work.is_contiguous() else 0
             if have < n:
-                raise ValueError(f"{what}: work holds {have} bytes, the call needs {n}")
+                raise ValueError(f"{what}: work holds {have} dense bytes, the call needs {n}")
         pw = work.data_ptr()
     args = _pack_attention(pq, po, pt, pl, ps, pv, pw, have, rows, ldq, ldo, seqs, max_pages, max_q, heads, dtype, scale)
     _check(l.vda_cached_attention(desc, args, _stream()), what)

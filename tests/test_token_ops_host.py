@@ -332,3 +332,44 @@ def test_a_row_stride_that_is_given_counts_from_the_tensors_first_element(addres
     for bad in (buf[2 * WIDTH + 8:], torch.zeros(8 * ROWS, 2 * HD, dtype=f16)[:, :HD]):          # beyond the memory; a row that is not dense
         with pytest.raises(ValueError):
             hip.rotary_axes(bad, out, pos, freq, ldx=3 * WIDTH, **kw)
+
+
+def test_vectors_and_workspaces_end_where_the_tensor_does(addressed, monkeypatch):
+    """A tensor that is shorter than the call needs is refused, also where the memory behind it goes on: what lies there is another
+    tensor's (the next frame's gate, another call's workspace)."""
+    whole = lambda dtype: torch.zeros(64, WIDTH, dtype=dtype)  # noqa: E731
+    x, y, b = torch.zeros(ROWS, WIDTH), torch.zeros(ROWS, WIDTH, dtype=f16), torch.zeros(ROWS, WIDTH, dtype=f16)
+    norm = dict(rows=ROWS, C=WIDTH, rows_per_group=2)
+    gates, w = whole(f32)[:3], whole(f32)[0]
+    hip.gated_norm(x, b, x, y, gate=gates, mod_scale=gates, mod_shift=gates, post_w=w, post_b=w, pre_w=w, pre_b=w, **norm)
+    for name, t in (("gate", whole(f32)[0]), ("mod_scale", whole(f32)[:2]), ("mod_shift", whole(f32)[:2]), ("post_w", whole(f32)[0, :-1]), ("post_b", whole(f32)[0, :-1]),
+                    ("pre_w", whole(f32)[0, 1:]), ("pre_b", whole(f32)[0, 1:])):
+        with pytest.raises(ValueError, match=f"{name} holds"):
+            hip.gated_norm(x, b, x, y, **{name: t}, **norm)
+    pos, freq, slots = torch.zeros(64, 3, dtype=i32), torch.zeros(64, dtype=f64), torch.zeros(64, dtype=i64)
+    rot = dict(rows=ROWS, heads=HEADS, hd=HD, sections=(8, 12, 12))
+    hip.rotary_axes(b, y, pos[:ROWS], freq[:32], **rot)
+    for p, f, name in ((pos[:ROWS - 1], freq, "pos"), (pos, freq[:31], "freq")):
+        with pytest.raises(ValueError, match=f"{name} holds"):
+            hip.rotary_axes(b, y, p, f, **rot)
+    p = planes(heads=HEADS, hd=HD)
+    cache = dict(kv_heads=HEADS, hd=HD, page_size=16, fmt=hip.CACHE_I8)
+    for call in (lambda: hip.cache_write(b, y, *p, slots[:ROWS - 1], rows=ROWS, **cache), lambda: hip.cache_read(*p, slots[:ROWS - 1], b, y, rows=ROWS, **cache)):
+        with pytest.raises(ValueError, match="slots holds"):
+            call()
+    seq = torch.zeros(1, 3, dtype=i32), torch.zeros(1, dtype=i32), torch.zeros(2, dtype=i32)
+    att = dict(heads=HEADS, max_q=ROWS, scale=0.1, **cache)
+    with pytest.raises(ValueError, match="visible holds"):
+        hip.cached_attention(b, y, *p, *seq, visible=torch.zeros(64, dtype=i32)[:ROWS - 1], **att)
+
+    class Needs:
+        vda_cached_attention_work = staticmethod(lambda *a: 4096)
+        vda_cached_attention = staticmethod(lambda *a: 0)
+
+    monkeypatch.setattr(hip, "lib", lambda: Needs)
+    arena = torch.zeros(4 * 4096, dtype=u8)
+    hip.cached_attention(b, y, *p, *seq, work=arena[4096:8192], **att)
+    hip.cached_attention(b, y, *p, *seq, work=arena.view(f32)[:1024], **att)
+    for work in (arena[4096:8191], arena.view(f32)[:1023], arena[::2][:4096]):
+        with pytest.raises(ValueError, match="work"):
+            hip.cached_attention(b, y, *p, *seq, work=work, **att)

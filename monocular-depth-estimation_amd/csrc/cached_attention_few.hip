@@ -49,8 +49,9 @@ template <typename T, int HDP> constexpr int few_waves() {
 }
 
 // W waves share a (sequence, key head, row block, split) item, each with a part of its keys; W = 1: a wave per item.
+// (out may be q: each row's queries are read by the workgroup that writes it, before it writes)
 template <typename T, int HDP, int FMT, int W>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void attend_few_kernel(const T* __restrict__ q, T* __restrict__ out,
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, (few_waves<T, HDP>())) void attend_few_kernel(const T* q, T* out,
                                                                                                        AttendJob j, int max_q, int items) {
     constexpr int NP = Pieces<T>::n, C64 = HDP / 64, TAIL32 = (HDP / 32) & 1, CB = HDP / 32;
     constexpr int LD = HDP + 4, JOIN = W == 1 ? 0 : W * (LD * 16 + 32) * 4, TILES = (W == 1 ? 4 : W) * 32 * HDP;

@@ -76,8 +76,9 @@ __device__ __forceinline__ void scaled16(u32x4 w, int e, f16x8& lo, f16x8& hi) {
 // Waves per SIMD that the registers allow without spilling.
 template <typename T, int HDP> constexpr int many_waves() { return HDP <= 64 ? 3 : HDP == 128 && Pieces<T>::n == 2 ? 1 : 2; }
 
+// (out may be q: each row's queries are read by the workgroup that writes it, before it writes)
 template <typename T, int HDP, int FMT>
-__global__ __launch_bounds__(256, (many_waves<T, HDP>())) void attend_many_kernel(const T* __restrict__ q, T* __restrict__ out, AttendJob j, int max_q, int groups) {
+__global__ __launch_bounds__(256, (many_waves<T, HDP>())) void attend_many_kernel(const T* q, T* out, AttendJob j, int max_q, int groups) {
     constexpr int NP = Pieces<T>::n, KS = HDP / 16, DB = HDP / 32, CPR = HDP / 16, NC = (HDP + 63) / 64, SHIFT = FMT == VDA_CACHE_I8 ? 8 : 6;
     constexpr int PLANE = TK * HDP * 2, BUF = 2 * PLANE;
     __shared__ __attribute__((aligned(16))) char smem[2 * BUF];

@@ -373,3 +373,13 @@ def test_vectors_and_workspaces_end_where_the_tensor_does(addressed, monkeypatch
     for work in (arena[4096:8191], arena.view(f32)[:1023], arena[::2][:4096]):
         with pytest.raises(ValueError, match="work"):
             hip.cached_attention(b, y, *p, *seq, work=work, **att)
+
+
+def test_attention_kernels_do_not_promise_that_queries_and_outputs_lie_apart():
+    """`out` may be `q`: a __restrict__ on either would let the compiler read q after it has written out."""
+    import re
+    csrc = os.path.join(ROOT, "monocular-depth-estimation_amd", "csrc")
+    for name in ("cached_attention_few.hip", "cached_attention_many.hip"):
+        heads = re.findall(r"void\s+(attend_(?:few|many)_kernel)\(([^)]*)\)", open(os.path.join(csrc, name)).read())
+        assert len(heads) == 1
+        assert "__restrict__" not in heads[0][1], heads

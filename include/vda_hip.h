@@ -406,7 +406,7 @@ int vda_cache_read(const VdaTokenCache* cache, const int64_t* slots, void* k, vo
  *   the first visible[r] of its sequence's keys (int32 [rows]; NULL: all): a causal mask, by token or by frame.  Keys
  *   in empty slots and in pages outside 0 .. pages-1 (evicted ones: -1) are not seen by any row.  A row that sees no key is 0.  What
  *   is not seen has no effect on a row, NaN and values of any size included (other rows' keys may change which way a result rounds).
- *   Query heads h * G .. h * G + G-1 use key head h, G = heads / kv_heads.
+ *   Query heads h * G .. h * G + G-1 use key head h, G = heads / kv_heads.  scale is finite, of any sign.
  *   q, out: dtype BF16, F16 or F32, rows of ldq and ldo elements, 16-byte aligned (out may be q itself, with ldo == ldq, and must not
  *   overlap it otherwise); rows of no sequence are left as they were.
  *   Scores, softmax and sums are fp32 (keys beyond 1e29 overflow them, values below 1e-30 lose bits).  16-bit types: products of IEEE

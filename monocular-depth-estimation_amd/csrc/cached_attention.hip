@@ -2,6 +2,8 @@
 // (see vda_cached_attention in include/vda_hip.h).
 #include "cached_attention.h"
 
+#include <cmath>
+
 namespace {
 
 struct Plan {
@@ -84,6 +86,8 @@ extern "C" long vda_cached_attention_work(const VdaTokenCache* cache, int seqs, 
 extern "C" int vda_cached_attention(const VdaTokenCache* cache, const VdaCachedAttentionArgs* a, void* stream) {
     if (!a || !a->q || !a->out || !a->page_table || !a->kv_len || !a->q_start || a->rows <= 0) return VDA_EINVAL;
     if (a->dtype != VDA_T_BF16 && a->dtype != VDA_T_F16 && a->dtype != VDA_T_F32) return VDA_EINVAL;
+    const float octaves = a->scale * 1.4426950408889634f;
+    if (!std::isfinite(octaves)) return VDA_EINVAL;
     Plan p;
     if (const int rc = plan_of(cache, a->seqs, a->max_pages, a->max_q, a->heads, &p)) return rc;
     const int size = a->dtype == VDA_T_F32 ? 4 : 2;
@@ -96,7 +100,7 @@ extern "C" int vda_cached_attention(const VdaTokenCache* cache, const VdaCachedA
     }
     const AttendJob j{(const uint8_t*)cache->k, (const uint8_t*)cache->v, cache->k_exp, cache->v_exp, a->page_table, a->kv_len, a->q_start, a->visible,
                       (float*)a->work, a->rows, a->ldq, a->ldo, cache->pages, cache->page_size, cache->kv_heads, cache->hd, cache_row_bytes(cache->hd),
-                      a->max_pages, a->heads / cache->kv_heads, a->seqs, p.row_blocks, p.splits, p.chunk, a->scale * 1.4426950408889634f,
+                      a->max_pages, a->heads / cache->kv_heads, a->seqs, p.row_blocks, p.splits, p.chunk, octaves,
                       Quick(p.splits), Quick(cache->kv_heads), Quick(p.row_blocks), Quick(a->heads / cache->kv_heads), Quick(cache->page_size)};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int rc = p.waves ? attend_few(j, a->q, a->out, a->dtype, cache->format, a->max_q, p.waves, st)

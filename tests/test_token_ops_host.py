@@ -383,3 +383,10 @@ def test_attention_kernels_do_not_promise_that_queries_and_outputs_lie_apart():
         heads = re.findall(r"void\s+(attend_(?:few|many)_kernel)\(([^)]*)\)", open(os.path.join(csrc, name)).read())
         assert len(heads) == 1
         assert "__restrict__" not in heads[0][1], heads
+
+
+def test_c_attention_refuses_a_scale_that_is_no_number():
+    """One kernel would take it for 0, the other give NaN."""
+    f = hip.lib().vda_cached_attention
+    for scale in (float("nan"), float("inf"), -float("inf"), 3e38):
+        assert f(ctypes.byref(desc()), ctypes.byref(attention_args(scale=scale)), None) == EINVAL, scale

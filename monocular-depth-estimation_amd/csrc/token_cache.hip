@@ -171,12 +171,12 @@ __device__ __forceinline__ int exponent_byte(unsigned amax_bits, int format) {
     const unsigned mant = amax_bits & 0x7fffff;
     if (field == 255) return 255;                                  // the row holds an infinity or a NaN
     const int e = format == VDA_CACHE_I8 ? field - 6 + (mant > 0x7e0000) : field - 8 + (mant > 0x600000);
-    return max(1, min(254, e));                                    // 0 marks an empty slot
+    return max(1, e);                                              // 0 marks an empty slot; 249 at most (254 - 6 + 1)
 }
 __device__ __forceinline__ u32x2 encode8(const float* f, int byte, int format) {
     u32x2 c = {0u, 0u};
     if (byte == 255) return c;
-    const float s = byte == 254 ? __uint_as_float(1u << 22) : __uint_as_float((unsigned)(254 - byte) << 23);      // 2^(127 - byte)
+    const float s = __uint_as_float((unsigned)(254 - byte) << 23);      // 2^(127 - byte)
     if (format == VDA_CACHE_I8) {
         // on 1.5 * 2^23 a unit in the last place is 1: the sum's one rounding, to nearest even, leaves the code in the low byte
 #pragma unroll

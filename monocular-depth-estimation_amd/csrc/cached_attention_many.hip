@@ -31,7 +31,7 @@ constexpr int TK = 64;                                            // keys of a t
 // a value 2^8 larger than another.
 template <int FMT> constexpr int key_spread() { return FMT == VDA_CACHE_I8 ? 32 : 21; }
 constexpr int VALUE_SPREAD = 8;
-constexpr int V_MIN = 40;            // of single exponents, smaller ones of values count as this (see V_REF_MIN in the kernel for few rows)
+constexpr int V_MIN = 40;            // smaller value exponents count as this where they are part of a reference (see V_REF_MIN in the kernel for few rows)
 
 __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
@@ -384,7 +384,8 @@ __global__ __launch_bounds__(256, (many_waves<T, HDP>())) void attend_many_kerne
         float* d = part + in_wg * HDP + 4 * h;
         // as the join expects them: outputs and sum relative to one power of two, which holds the value exponent; what its rounding leaves out
         // (a hundred thousandth) multiplies both
-        const float v = (float)v_ref, m = unset ? LOWEST : m_run + v, v_in = m - m_run;
+        const int v_in_m = max(v_ref, V_MIN);                     // (a smaller one would make the sum overflow)
+        const float v = (float)v_in_m, m = unset ? LOWEST : m_run + v, v_in = m - m_run;
         const float left = unset ? 1.f : __builtin_amdgcn_exp2f((m_run - (m - v_in)) + (v - v_in));
 #pragma unroll
         for (int i = 0; i < DB; ++i)
@@ -392,12 +393,12 @@ __global__ __launch_bounds__(256, (many_waves<T, HDP>())) void attend_many_kerne
             for (int g = 0; g < 4; ++g) {
                 f32x4 y;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) y[x] = __builtin_amdgcn_ldexpf(o[i][4 * g + x] * left, -SHIFT);
+                for (int x = 0; x < 4; ++x) y[x] = __builtin_amdgcn_ldexpf(o[i][4 * g + x] * left, v_ref - v_in_m - SHIFT);
                 *reinterpret_cast<f32x4*>(d + 32 * i + 8 * g) = y;
             }
         if (h == 0) {
             part[128 * HDP + in_wg] = m;
-            part[128 * HDP + 128 + in_wg] = __builtin_amdgcn_ldexpf(l * left, 127 - v_ref);
+            part[128 * HDP + 128 + in_wg] = __builtin_amdgcn_ldexpf(l * left, 127 - v_in_m);
         }
         return;
     }

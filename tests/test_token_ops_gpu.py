@@ -825,3 +825,17 @@ def test_attention_with_tiny_and_huge_values(q_len, kv, table_pages, size, dt, f
     k, v = torch.randn((kv, 32), generator=g), torch.randn((kv, 32), generator=g)
     store(m, list(range(kv)), k, v * size)
     m.check(queries(q_len, 1, 32, dt, 203), [0, q_len], 1)
+
+
+@pytest.mark.parametrize("dt,fmt", WIDE)
+@pytest.mark.parametrize("size", [0.0, 1e-37])
+@pytest.mark.parametrize("q_len,kv,table_pages", [(1, 6000, 0), (9, 700, 0), (70, 3000, 300), (200, 1500, 300)])
+def test_attention_parts_whose_values_are_zeros_join_parts_whose_values_are_not(q_len, kv, table_pages, size, dt, fmt):
+    """A part of the key axis without any value to speak of weighs in the sum of probabilities as every other."""
+    m = Memory([kv], 1, 32, 16, fmt, 211)
+    m.table = torch.nn.functional.pad(m.table, (0, max(0, table_pages - m.table.shape[1])), value=-1)
+    g = gen(212)
+    k, v = torch.randn((kv, 32), generator=g), torch.randn((kv, 32), generator=g)
+    v[:kv // 2] *= size
+    store(m, list(range(kv)), k, v)
+    m.check(queries(q_len, 1, 32, dt, 213), [0, q_len], 1)

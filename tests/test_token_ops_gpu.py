@@ -839,3 +839,31 @@ def test_attention_parts_whose_values_are_zeros_join_parts_whose_values_are_not(
     v[:kv // 2] *= size
     store(m, list(range(kv)), k, v)
     m.check(queries(q_len, 1, 32, dt, 213), [0, q_len], 1)
+
+
+@pytest.mark.parametrize("dt,fmt", WIDE)
+@pytest.mark.parametrize("spread", [0, 20])
+@pytest.mark.parametrize("q_len,kv", [(40, 150), (150, 1300)])
+def test_attention_many_rows_nan_rows_empty_slots_and_evicted_pages(q_len, kv, spread, dt, fmt):
+    """The kernel for many rows, in its form for neighbouring exponents and in the one for others: a NaN row is seen by the rows that reach
+    it, and by no other; empty slots and absent pages by none."""
+    m = Memory([kv, 33], 2, 64, 16, fmt, 221)
+    g = gen(222)
+    v = torch.randn((kv, 64), generator=g) * torch.exp2(torch.randint(-spread // 2, spread // 2 + 1, (kv, 1), generator=g).float())
+    store(m, list(range(kv)), torch.randn((kv, 64), generator=g), v)
+    m.planes[2].view(-1)[::7] = 0
+    m.table = torch.nn.functional.pad(m.table, (0, 300), value=-1)
+    m.table[0, 4], m.table[0, 5] = -1, m.planes[0].shape[0]
+    start = [0, q_len, q_len + 3]
+    visible = torch.cat([torch.arange(q_len) + kv - q_len + 1, torch.tensor([33, 0, 20])]).int()
+    q = queries(q_len + 3, 4, 64, dt, 223)
+    out, want, rows = m.check(q, start, 4, visible=visible)
+    assert bool((out[q_len + 1] == 0).all())
+    at = kv - q_len // 2
+    for k, v in ((math.nan, 1.0), (1.0, math.inf)):
+        store(m, [at], torch.full((1, 64), k), torch.full((1, 64), v))
+        again, want, tol, _ = m.attend(q, start, 4, visible=visible)
+        sees = visible > at
+        sees[q_len:] = False
+        assert bool(torch.isnan(again[sees.to(DEV)]).all())
+        within(again[~sees.to(DEV)], want[~sees], tol[~sees])

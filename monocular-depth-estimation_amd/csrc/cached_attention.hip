@@ -29,6 +29,8 @@ constexpr int MIN_PART = 512;        // keys of a part at least
 // Tried: parts that make 256, 512, ... 2048 workgroups.  Measured, us of 1 part / 512 / 1024 / 2048 workgroups on the device, heads of 64:
 // 64 items of 10960 keys 60 / 28 / 35 / 40, 192 items 71 / 61 / 58 / 62, 256 items of 4096 keys 29 / 31 / 34 / 41, 512 items of 10960
 // keys 147 / - / 155 / 159; 6 items of 3000 keys 18.8, in six parts 10.1; heads of 128: 192 items of 10960 keys 114 / 132 / 126 / 137.
+// The rule does not know how many bytes a key has: at 32 channels it leaves 384 items of 10960 keys in one part, 83 us, where parts
+// took 72.  It goes by the keys that the table can hold, as the workspace does: a table wider than its sequences may cost a join.
 long part_of(long keys, long items, bool wide) {
     long best = 0, part = keys;
     for (int j = 0; j <= 8; ++j) {

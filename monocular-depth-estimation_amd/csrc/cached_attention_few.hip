@@ -15,8 +15,8 @@
 // depend on what its neighbours see.
 //
 // Measured: one token for each of 48 streams over one to eight frames of 1370 tokens, 16 query heads on 4 key heads of 64 (170 MB),
-// 41 us here, 4.1 TB/s, and 4.7 us in the join; one token for each of 5476 positions over 32 keys, 8 heads of 32 (98 MB), 29 us,
-// 3.4 TB/s: there a wave lives for one step and its chain of loads (arguments, page, keys) is what it lasts.
+// 42 us here, 4.0 TB/s, and 4.6 us in the join; one token for each of 5476 positions over 32 keys, 8 heads of 32 (98 MB), 30 us,
+// 3.3 TB/s: there a wave lives for one step and its chain of loads (arguments, page, keys) is what it lasts.
 #include "cached_attention.h"
 
 namespace {

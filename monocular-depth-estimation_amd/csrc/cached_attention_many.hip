@@ -5,10 +5,11 @@
 // are stored in LDS once for the four waves, in a second buffer: one barrier per tile.  Scores are S^T = K Q^T (mfma 32x32x16), so a
 // query lives on a lane, the softmax needs one exchange (lane ^ 32) and only where a maximum grows, and the probabilities
 // are as they stand the B operand of O^T += V^T P^T, whose V^T operand the transposed LDS read gathers in the same key order.
-// What bounds it is vector instruction issue: about five instructions per score, one of them the exponential, against two matrix
-// instructions of 32 cycles per 1024 scores and 16 channels.  The 1370 tokens of a frame over 32 frames, 16 heads of 64: 375 us
-// (416 on a slower card), 0.66 PFLOP/s, where a large library product of the type reaches 1.2.  Vector and matrix instructions of different waves take
-// turns at the issue, so a fourth wave per SIMD (32 keys per tile) gains nothing: 388 us.  Within a wave, the scores of one half of the
+// What it spends its time on are vector instructions: about five per score, one of them the exponential, against two matrix
+// instructions of 32 cycles per 1024 scores and 16 channels.  The 1370 tokens of a frame over 32 frames, 16 heads of 64: 382 us
+// (433 where the clock is lower), 0.65 PFLOP/s, where a large library product of the type reaches 1.2.  Counters: a SIMD issues vector
+// instructions in 55 % of the cycles and its matrix pipe works in 27 %; of the 2.1 waves that it holds on average each waits for
+// memory or the barrier for 26 % of its time and for its turn to issue for 32 %.  A fourth wave per SIMD (32 keys per tile) gained nothing: 388 against 381 us.  Within a wave, the scores of one half of the
 // tile formed between the exponentials of the other: 1 % less here, 3 % more for three clips of 5 x 380 tokens, not kept; the
 // scores of the next tile between them: 204 registers, two waves, 607 us.  64 rows per wave: slower.
 //

@@ -123,7 +123,8 @@ __global__ __launch_bounds__(256) void rotary_line_kernel(const T* x, T* out, Ax
 }
 
 // The general form, for pairs in halves whose distance is no power of two pieces, and rows that are only 8-byte aligned: a
-// thread holds four pairs, or CU channels that are only copied.
+// thread holds four pairs, or CU channels that are only copied.  q and k of 32 x 1370 tokens, 16 + 16 heads of 64 of which 48 channels
+// turn: 103 us in bf16 (3.5 TB/s), 202 in fp32, where the line form takes 75 and 147 for whole heads; 20 heads of 96, all of it, 77 and 139.
 template <typename T>
 __global__ __launch_bounds__(256) void rotary_pairs_kernel(const T* x, T* out, Axes ax, RotaryShape s) {
     extern __shared__ float2 cs[];

@@ -30,6 +30,9 @@ __device__ __forceinline__ Span span_of(const AttendJob& j, int s, int max_q) {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 constexpr float LOWEST = -1e30f;        // running maximum of a row that has seen no key: exp2(-inf - LOWEST) is 0, not NaN
 constexpr float DEFER = 6.f;            // growth of the running maximum (in octaves) below which sums are not rescaled
+// Probabilities of 16-bit rows are one half each, 11 bits: that adds a tenth to a quarter to the error of an fp16 result (2.07e-4 of the
+// outputs becomes 2.2e-4 to 2.5e-4) and nothing to a bf16 one (1.6e-3).  Two pieces are what fp32 rows take, of q and of the
+// probabilities: 94 us where 16-bit rows take 67 (1370 rows over 10960 keys, 8 heads of 64).
 constexpr int P_SHIFT = 8;              // probabilities reach 2^DEFER; in IEEE halves they are kept times 2^P_SHIFT, far from subnormals
 
 // 8-bit codes to IEEE halves, exactly.  Integers: the biased byte under the exponent of 1024, then minus 1024 + 128.
